@@ -476,6 +476,61 @@ int lssvc_engine_decode_pframe(void *engine, const uint8_t *bl_file, int64_t bl_
                                const float *ref_frame_bl, const float *ref_frame_el, const float *ref_feature_bl, const float *ref_feature_el,
                                float *recon_bl, float *feature_bl, float *recon_el, float *feature_el, void *stream);
 
+/* ---- row operators: typed, batched rows ------------------------------------------------------------------------------------
+ * A row matrix is what a channels-last map of any batch is: rows = images x H x W, cols = C, `ld` elements between rows. These
+ * operators have no counterpart in the reference; they serve transform blocks that normalise over channel groups and take their
+ * pointwise products in 8 bits. They are not part of compiled frame plans. */
+enum { LSSVC_F32 = 0, LSSVC_F16 = 1, LSSVC_BF16 = 2 };
+#define LSSVC_ACT_SILU 3 /* x / (1 + exp(-x)); row operators only, beside LSSVC_ACT_* */
+
+typedef struct lssvc_rows {
+    void *ptr;      /* device pointer, aligned to the element */
+    int64_t rows;
+    int64_t ld;     /* elements between rows (>= cols) */
+    int32_t cols;
+    int32_t dtype;  /* LSSVC_F32 ... */
+} lssvc_rows;
+
+/* 8-bit rows with a scale for each block of block_rows x 128 values: value (r, c) stands for
+ * e4m3(values[r * ld + c]) * scale[(r / block_rows) * scale_ld + c / 128] (OCP e4m3: 4 exponent bits, 3 mantissa bits, largest 448).
+ * values: 16-byte aligned, ld a multiple of 16; the bytes of columns cols ... next multiple of 16 are zero in every row.
+ * Scales: e8m0 (scale_e8m0 = 1: one byte b stands for 2^(b - 127), 255 for NaN; 4-byte aligned, scale_ld a multiple of 4) or
+ * fp32 (scale_e8m0 = 0). */
+typedef struct lssvc_fp8 {
+    void *values;
+    void *scale;
+    int64_t rows;
+    int64_t ld;
+    int64_t scale_ld;
+    int32_t cols;
+    int32_t block_rows; /* 1 or 128 */
+    int32_t scale_e8m0;
+    int32_t reserved;   /* 0 */
+} lssvc_fp8;
+
+/* Group norm over channel groups, with an activation: per image and group of cols / groups channels
+ *   y = act((x - mean) / sqrt(mean((x - mean)^2) + eps) * weight[c] + bias[c]),   statistics in fp32, two-level and shifted.
+ * x holds images x (rows / images) rows. weight / bias: cols fp32 values or NULL (1 / 0). Exactly one of y (x's shape and type;
+ * may be x itself) and y8 (1 x 128 blocks, e8m0 scales; the block's scale and values are those lssvc_quantize_fp8 makes of the
+ * fp32 result) is given. rows = 0 is no work. workspace: lssvc_group_norm_workspace_bytes(...) bytes, 16-byte aligned, private to
+ * the call until it has run; may be NULL where that is 0. */
+int64_t lssvc_group_norm_workspace_bytes(int64_t rows, int32_t images, int32_t cols, int32_t groups, int32_t dtype, int32_t to_fp8);
+int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t groups, const float *weight, const float *bias, float eps,
+                     int32_t act, float slope, const lssvc_rows *y, const lssvc_fp8 *y8, void *workspace, int64_t workspace_bytes,
+                     void *stream);
+
+/* x -> 8-bit rows (y->block_rows 1: activations; 128: weights), e8m0 scales: of each block the smallest power of two s >= 2^-126
+ * with max |x| <= 448 s (1 where the block is zero), values e4m3(x / s) to nearest even. A value that is not finite becomes NaN
+ * and does not move the scale. Writes the zero bytes behind the last column. */
+int lssvc_quantize_fp8(const lssvc_rows *x, const lssvc_fp8 *y, void *stream);
+
+/* y[m][n] = act(sum_k a[m][k] w[n][k] + bias[n]) + residual[m][n], sums in fp32. a: block_rows 1; w: block_rows 128; both with e8m0
+ * scales (applied by the matrix instruction) or both with fp32 scales (applied to each 128-block's partial sum). bias: w->rows fp32
+ * values or NULL. residual: y's shape and type or NULL; may be y itself. a->rows = 0 is no work. workspace: as above. */
+int64_t lssvc_matmul_fp8_workspace_bytes(int64_t m, int64_t n, int32_t k);
+int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const float *bias, int32_t act, float slope, const lssvc_rows *residual,
+                     const lssvc_rows *y, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* Runtime tuning switches (each also reads an environment variable at first use):
  *   "f16x3_persist"            1/0   use the persistent warp-specialised 3x3 kernel (LSSVC_F16X3_PERSIST)
  *   "f16x3_persist_min_tiles"  n     ... for convs with at least n output tiles (LSSVC_F16X3_PERSIST_MIN_TILES, 256)

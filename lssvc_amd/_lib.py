@@ -16,7 +16,8 @@ LIB_PATH = os.environ.get("LSSVC_HIP_LIB") or os.path.join(_HERE, "lib", "liblss
 CONV_MAX_INPUTS = 3
 CONV_CK = 8
 
-ACT_NONE, ACT_LRELU, ACT_RELU = 0, 1, 2
+ACT_NONE, ACT_LRELU, ACT_RELU, ACT_SILU = 0, 1, 2, 3      # SILU: row operators only
+F32, F16, BF16 = 0, 1, 2
 INACT_NONE, INACT_LRELU, INACT_SQUARE = 0, 1, 2
 PREC_F32, PREC_F16X3 = 0, 1
 PREC_MASK, PREC_SPLIT_IN = 0xff, 0x100
@@ -51,6 +52,15 @@ class FfnDesc(C.Structure):
     ]
 
 
+class Rows(C.Structure):
+    _fields_ = [("ptr", C.c_void_p), ("rows", C.c_int64), ("ld", C.c_int64), ("cols", C.c_int32), ("dtype", C.c_int32)]
+
+
+class Fp8(C.Structure):
+    _fields_ = [("values", C.c_void_p), ("scale", C.c_void_p), ("rows", C.c_int64), ("ld", C.c_int64), ("scale_ld", C.c_int64),
+                ("cols", C.c_int32), ("block_rows", C.c_int32), ("scale_e8m0", C.c_int32), ("reserved", C.c_int32)]
+
+
 class CdfTable(C.Structure):
     _fields_ = [("cdfs", C.c_void_p), ("n_cdfs", C.c_int32), ("stride", C.c_int32), ("sizes", C.c_void_p),
                 ("offsets", C.c_void_p)]
@@ -69,6 +79,8 @@ PREP_CONV, PREP_CONV_F16X3, PREP_CONVT, PREP_DWCONV, PREP_GDN, PREP_VECTOR, PREP
 PREP_MAX_BLOBS = 8
 
 VP = C.POINTER(View)
+RP = C.POINTER(Rows)
+FP = C.POINTER(Fp8)
 TP = C.POINTER(CdfTable)
 
 # name -> (restype, argtypes); every symbol include/lssvc_hip.h declares
@@ -149,6 +161,11 @@ SIGNATURES = {
     "lssvc_engine_decode_iframe": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64] + [C.c_void_p] * 4),
     "lssvc_engine_encode_pframe": (C.c_int, [C.c_void_p] * 8 + [C.c_int64, C.POINTER(C.c_int64), C.c_void_p, C.c_int64, C.POINTER(C.c_int64)] + [C.c_void_p] * 5),
     "lssvc_engine_decode_pframe": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64] + [C.c_void_p] * 9),
+    "lssvc_group_norm_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "lssvc_group_norm": (C.c_int, [RP, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_float, C.c_int32, C.c_float, RP, FP, C.c_void_p, C.c_int64, C.c_void_p]),
+    "lssvc_quantize_fp8": (C.c_int, [RP, FP, C.c_void_p]),
+    "lssvc_matmul_fp8_workspace_bytes": (C.c_int64, [C.c_int64, C.c_int64, C.c_int32]),
+    "lssvc_matmul_fp8": (C.c_int, [FP, FP, C.c_void_p, C.c_int32, C.c_float, RP, RP, C.c_void_p, C.c_int64, C.c_void_p]),
     "lssvc_set_option": (C.c_int, [C.c_char_p, C.c_int32]),
     "lssvc_get_option": (C.c_int, [C.c_char_p, C.POINTER(C.c_int32)]),
     "lssvc_last_error": (C.c_char_p, []),

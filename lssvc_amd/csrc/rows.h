@@ -1,0 +1,91 @@
+// Shared device helpers of the row operators (group norm, block quantiser, 8-bit product): typed rows, activations, 8-bit encoding.
+#pragma once
+#include "common.h"
+
+namespace lssvc {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kFp8Block = 128;   // columns that share a scale
+
+inline bool rows_type_ok(int t) { return t == LSSVC_F32 || t == LSSVC_F16 || t == LSSVC_BF16; }
+inline int rows_type_size(int t) { return t == LSSVC_F32 ? 4 : 2; }
+inline bool act_ok(int a) { return a >= LSSVC_ACT_NONE && a <= LSSVC_ACT_SILU; }
+inline bool aligned(const void *p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// Two row matrices either share no byte, or are the very same one: a channel slice beside another slice of the same wide buffer
+// overlaps as an address range and is fine; anything in between would be read after it was written.
+inline bool rows_disjoint_or_same(const lssvc_rows *a, const lssvc_rows *b) {
+    const int sa = rows_type_size(a->dtype), sb = rows_type_size(b->dtype);
+    const uintptr_t pa = (uintptr_t)a->ptr, pb = (uintptr_t)b->ptr;
+    const uint64_t wa = (uint64_t)a->cols * sa, wb = (uint64_t)b->cols * sb, la = (uint64_t)a->ld * sa, lb = (uint64_t)b->ld * sb;
+    const uintptr_t ea = pa + (uint64_t)(a->rows - 1) * la + wa, eb = pb + (uint64_t)(b->rows - 1) * lb + wb;
+    if (ea <= pb || eb <= pa) return true;
+    if (la != lb) return false;
+    if (pa == pb) return a->dtype == b->dtype;
+    const uint64_t d = pb > pa ? (pb - pa) % la : (la - (pa - pb) % la) % la;       // where b's columns start within a's pitch
+    return d >= wa && d + wb <= la;
+}
+
+// ---- typed values: every kernel computes in fp32; storing to 16 bits is the one rounding (to nearest even) ----------------------
+struct bf16_t { uint16_t v; };
+struct f16_t { _Float16 v; };
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(f16_t x) { return (float)x.v; }
+__device__ __forceinline__ float to_f32(bf16_t x) { return __uint_as_float((uint32_t)x.v << 16); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ f16_t from_f32<f16_t>(float x) { return f16_t{(_Float16)x}; }
+template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float x) {
+    const __bf16 b = (__bf16)x;
+    return bf16_t{__builtin_bit_cast(uint16_t, b)};
+}
+
+// N consecutive values as they lie in memory, at the type's own alignment: global loads and stores of any width need no more on
+// gfx950, so slices and odd pitches take the wide path too.
+template <typename T, int N> struct Pack { T v[N]; };
+template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
+    Pack<T, N> r;
+    __builtin_memcpy(&r, p, sizeof(r));
+    return r;
+}
+template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) { __builtin_memcpy(p, &r, sizeof(r)); }
+
+// exp and reciprocal at the hardware's 1 ulp: 2^-22 relative beside the 2^-24 .. 2^-8 of the stored result. NaN passes through all.
+__device__ __forceinline__ float apply_act(float v, int act, float slope) {
+    if (act == LSSVC_ACT_NONE) return v;
+    if (act == LSSVC_ACT_LRELU) return v >= 0.f ? v : v * slope;
+    if (act == LSSVC_ACT_RELU) return v < 0.f ? 0.f : v;
+    return v * __builtin_amdgcn_rcpf(1.f + __expf(-v));
+}
+
+// ---- 8-bit blocks ---------------------------------------------------------------------------------------------------------------
+// max over the 16 lanes of a DPP row; every lane gets it
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, true));   // row_ror:8
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, true));
+    v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
+}
+// |x| as an ordered integer; what is not finite counts as 0 and does not move a scale
+__device__ __forceinline__ uint32_t finite_abs_bits(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
+// The exponent byte of the smallest power of two s >= 2^-126 with amax <= 448 s (1 where amax = 0). amax = m 2^k with m in [0.5, 1)
+// and 448 = 0.875 * 2^9, so s = 2^(k - 9) where m <= 0.875 and 2^(k - 8) otherwise; k = field - 126.
+__device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax_bits) {
+    if (amax_bits == 0u) return 127u;
+    const int field = (int)(amax_bits >> 23), e = field - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return (uint32_t)(e < 1 ? 1 : e);
+}
+__device__ __forceinline__ float scale_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }   // 2^-(byte - 127), byte <= 247: exact
+// four values that lie within +-448 (or are not finite: NaN) to e4m3, to nearest even
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+}  // namespace lssvc
