@@ -25,8 +25,8 @@ struct MatmulP {
     void *y;
     int64_t ldres, ldy;
     int M, N, K16, nkb;      // K16: bytes of a row that are read (K rounded up to 16; zeros behind K)
-    int dtype, act;
-    float slope;
+    int dtype;
+    Act act;
     int tiles_m, tiles_n;
 };
 
@@ -91,8 +91,7 @@ __device__ __forceinline__ void store_cols(const MatmulP &p, int64_t m, int n, f
     T *dst = (T *)p.y + m * p.ldy + n;
     const T *res = p.res ? (const T *)p.res + m * p.ldres + n : nullptr;
     const bool full = n + CNT <= p.N;
-#pragma unroll
-    for (int i = 0; i < CNT; ++i) v[i] = apply_act(v[i], p.act, p.slope);
+    apply_act(v, p.act);
     if (res) {
         Pack<T, CNT> r;
         if (full) r = load_pack<T, CNT>(res);
@@ -398,6 +397,6 @@ extern "C" int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const fl
     p.res = residual ? residual->ptr : nullptr, p.ldres = residual ? residual->ld : 0;
     p.y = y->ptr, p.ldy = y->ld;
     p.M = (int)a->rows, p.N = (int)w->rows, p.K16 = (a->cols + 15) / 16 * 16, p.nkb = (a->cols + kFp8Block - 1) / kFp8Block;
-    p.dtype = y->dtype, p.act = act, p.slope = slope;
+    p.dtype = y->dtype, p.act = make_act(act, slope);
     return a->scale_e8m0 ? launch_typed<true>(p, (hipStream_t)stream) : launch_typed<false>(p, (hipStream_t)stream);
 }

@@ -3,15 +3,19 @@
 // y = act((x - mu) * rsqrt(var + eps) * w_c + b_c), mu / var over the rows of an image and the cg = C / G channels of a group. The
 // operator is bound by memory: one read and one write of the map if it stays on the chip between the statistics and their use, two reads
 // otherwise. Two forms:
-//   resident  a workgroup owns all rows of a slice of whole groups and holds the slice in registers (up to 256 KB): one read, one write,
-//             one launch.
+//   resident  a workgroup owns all rows of a slice of whole groups and holds the slice in the LDS (up to 128 KB; every thread reads back
+//             what it wrote itself): one read, one write, one launch.
 //   split     rows are split over workgroups that write (mean, M2) per chunk and group; one wave per group merges the chunks; the
 //             normalising pass reads the map again, in the opposite order, so that what the first pass read last comes from the caches.
 // Every sum is taken of differences to a value of the group itself (a pivot), and squares of differences to a mean, never E[x^2] - E[x]^2:
 // a map whose offset is a thousand times its spread keeps the digits of its spread.
 //
-// One thread handles 8 consecutive channels (16 or 32 bytes, at any alignment). Where 8 does not divide the slice, a row's last thread
-// loads the LAST 8 channels -- wide loads only -- and owns those that its neighbour does not.
+// One thread handles V consecutive channels: 16 bytes at any alignment (8 channels where 8-bit blocks are written). Where V does not divide
+// the slice, a row's last thread loads the LAST V channels -- wide loads only -- and owns those that its neighbour does not (a slice of fewer
+// than V channels takes V = 1). An integer division costs about 40 instructions: a thread's place and its first group come from one
+// multiplication each.
+#include <algorithm>
+#include <type_traits>
 #include "rows.h"
 
 namespace lssvc {
@@ -23,91 +27,120 @@ struct NormP {
     int64_t ldx, ldy, ldq, ldqs;
     int64_t R;                   // rows of an image
     const float *w, *b;
-    float2 *part, *stat;         // split form: [image][chunk][unit] (mean, M2); [image][group] (mean, 1 / sqrt(var + eps))
+    float2 *part, *stat;         // split form: [image][chunk][unit] (mean, M2); [image][channel] (mean, weight / sqrt(var + eps))
     int64_t chunk;               // rows of a chunk
     int C, G, cg;
     int S;                       // chunks of an image
-    int P;                       // pieces of a group (1, or slices of kSliceMax where a group is wider than that)
+    int P, piece;                // pieces of a group: 1, or `piece` columns each where a group is wider than a workgroup takes
     int slice, nslices;          // columns of a slice (P = 1), slices of a row
-    int act;
-    float eps, slope;
+    Act act;
+    float eps;
+    int in_place;                // y is x: a row's last thread stores its own channels only
+    int nv;                      // threads of a row of a full slice; multiplications that divide by it, by a unit's width and by its share of a row
+    uint32_t m_nv, m_uw, m_w;
 };
 
-constexpr int kVec = 8;
-constexpr int kSliceMax = 2048;
+constexpr int kSliceMax = 1024;  // columns of a slice in the split form: 256 threads x 4; 256 where V = 1
+template <typename T> constexpr int kVecOf = 16 / (int)sizeof(T);
 
-// a thread's 8 channels of a slice that is `sc` columns wide
-struct Lane {
-    int cv, rt;        // which 8 channels, which of the rows in flight
+// a thread's V channels of a slice that is `sc` columns wide
+template <int V> struct Lane {
+    int cv, rt;        // which V channels, which of the rows in flight
     int lo;            // first channel that is loaded
     int own;           // loaded channels from `own` on are this thread's (below `end`)
     int end;
     bool live;
-    __device__ __forceinline__ Lane(int t, int nv, int rp, int sc) {
-        rt = t / nv;
+    __device__ __forceinline__ Lane(int t, int nv, uint32_t m_nv, int rp, int sc) {
+        rt = divided(t, m_nv);
         cv = t - rt * nv;
         live = rt < rp;
-        const int c0 = cv * kVec;
-        lo = sc >= kVec ? min(c0, sc - kVec) : 0;
+        const int c0 = cv * V;
+        lo = sc >= V ? min(c0, sc - V) : 0;
         own = c0 - lo;
-        end = sc >= kVec ? kVec : sc;
+        end = sc >= V ? V : sc;
         if (c0 >= sc) own = end = 0, lo = 0;         // padding lane of the 8-bit form: owns nothing
     }
     __device__ __forceinline__ bool owns(int j) const { return j >= own && j < end; }
+    // the unit (group, or piece) of each channel: units are `uw` wide and start at the slice's first column
+    template <bool ONE> __device__ __forceinline__ void units(int uw, uint32_t m_uw, int nu, int (&un)[V]) const {
+        int u = divided(lo, m_uw), c = lo - u * uw;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            un[j] = min(u, nu - 1);
+            if (!ONE && ++c == uw) c = 0, ++u;
+        }
+    }
 };
 
-template <typename T> __device__ __forceinline__ Pack<T, kVec> load_lane(const T *row, const Lane &l) {
-    if (l.end == kVec) return load_pack<T, kVec>(row + l.lo);
-    Pack<T, kVec> r;
+// threads of a row that is `sc` columns wide (the 8-bit form: 16 for every block of 128)
+template <int V, bool TO8> __host__ __device__ __forceinline__ int threads_of(int sc) {
+    return TO8 ? (sc + kFp8Block - 1) / kFp8Block * (kFp8Block / 8) : (sc + V - 1) / V;
+}
+
+template <typename T, int V, bool NARROW = false> __device__ __forceinline__ Pack<T, V> load_lane(const T *row, const Lane<V> &l) {
+    if (!NARROW || l.end == V) return load_pack<T, V>(row + l.lo);
+    Pack<T, V> r;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) r.v[j] = j < l.end ? row[l.lo + j] : from_f32<T>(0.f);
+    for (int j = 0; j < V; ++j) r.v[j] = j < l.end ? row[l.lo + j] : from_f32<T>(0.f);
     return r;
 }
 
-// Sums over (rows in flight x channels) per unit (a group, or a piece of one): v[j] is the thread's sum for channel lo + j. Entries go to
-// the LDS, each unit is added up by `lpu` lanes of one wave in a fixed order, totals come back in `tot`. ONE: 8 divides the unit width, so a
-// thread's channels lie in one unit and are added before.
-template <int TPB, bool ONE>
-__device__ __forceinline__ void unit_sums(const float (&v)[kVec], const Lane &l, int nv, int rp, int sc, int uw, int nu, float *ebuf, float *tot) {
+// Sums over (rows in flight x channels) per unit: v[j] is the thread's sum for channel lo + j. Entries go to the LDS, each unit is added up
+// by 2^sh lanes of one wave (all 64 unless there are more units than waves) in a fixed order, four reads in flight, and `done` makes of each
+// total what comes back in `tot`. ONE: V divides the unit width, so a thread's channels lie in one unit and are added before.
+template <int TPB, int V, bool ONE, typename F>
+__device__ __forceinline__ void unit_sums(const float (&v)[V], const Lane<V> &l, int nv, int rp, int sc, int uw, uint32_t m_w, int nu, float *ebuf, float *tot, F done) {
     const int t = threadIdx.x;
     if (l.live) {
         if constexpr (ONE) {
             float s = 0.f;
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) s += v[j];
+            for (int j = 0; j < V; ++j) s += v[j];
             ebuf[l.rt * nv + l.cv] = s;
         } else {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j)
+            for (int j = 0; j < V; ++j)
                 if (l.owns(j)) ebuf[l.rt * sc + l.lo + j] = v[j];
         }
     }
     __syncthreads();
-    const int W = ONE ? uw / kVec : uw, pitch = ONE ? nv : sc;
-    int lpu = 64;
-    while (lpu > 1 && lpu * nu > TPB) lpu >>= 1;
-    const int li = t & (lpu - 1), dr = lpu / W, dc = lpu - dr * W;
-    for (int u = t / lpu; u < nu; u += TPB / lpu) {
-        float s = 0.f;
-        int r = li / W, c = li - r * W;
+    const int W = ONE ? uw / V : uw, pitch = ONE ? nv : sc;
+    int sh = 6;
+    while (sh > 0 && (nu << sh) > TPB) --sh;
+    const int lpu = 1 << sh, li = t & (lpu - 1);
+    const int dr = divided(lpu, m_w), dc = lpu - dr * W;
+    const int r0 = divided(li, m_w), c0 = li - r0 * W;
+    for (int u = t >> sh; u < nu; u += TPB >> sh) {
+        float s[4] = {};
+        int r = r0, c = c0;
         while (r < rp) {
-            s += ebuf[r * pitch + u * W + c];
-            r += dr;
-            c += dc;
-            if (c >= W) c -= W, ++r;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const bool on = r < rp;
+                const float x = ebuf[on ? r * pitch + u * W + c : 0];
+                s[k] += on ? x : 0.f;
+                r += dr;
+                c += dc;
+                if (c >= W) c -= W, ++r;
+            }
         }
-        for (int o = lpu >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
-        if (li == 0) tot[u] = s;
+        float a = (s[0] + s[1]) + (s[2] + s[3]);
+        if (sh == 6) {
+            a = wave_sum_hi(a);
+            if (li == 63) tot[u] = done(u, a);
+        } else {
+            for (int o = lpu >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o);
+            if (li == 0) tot[u] = done(u, a);
+        }
     }
     __syncthreads();
 }
 
-// ---- split form, first pass: (mean, M2) of each chunk and unit ---------------------------------------------------------------------
-template <typename T, bool ONE>
+template <typename T, int V, bool ONE>
 __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
     constexpr int TPB = 256, NB = 4;
-    __shared__ float ebuf[TPB * kVec];
-    __shared__ float tot[kSliceMax], piv[kSliceMax];
+    __shared__ float ebuf[ONE ? TPB : TPB * V];
+    __shared__ float tot[kSliceMax], piv[kSliceMax], umean[kSliceMax];
     unsigned id = blockIdx.x;
     const int sl = id % (unsigned)p.nslices;
     id /= (unsigned)p.nslices;
@@ -120,30 +153,38 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
         nu = sc / uw;
     } else {
         const int g = sl / p.P, k = sl - g * p.P;
-        s0 = g * p.cg + k * kSliceMax;
-        sc = uw = min(kSliceMax, p.cg - k * kSliceMax);
+        s0 = g * p.cg + k * p.piece;
+        sc = uw = min(p.piece, p.cg - k * p.piece);
         nu = 1;
     }
-    const int nv = (sc + kVec - 1) / kVec, rp = TPB / nv, t = threadIdx.x;
-    const Lane l(t, nv, rp, sc);
+    int nv = p.nv;
+    uint32_t m_nv = p.m_nv, m_uw = p.m_uw, m_w = p.m_w;
+    if (sc != p.slice) nv = (sc + V - 1) / V, m_nv = division_magic(nv);           // the last slice; the last piece of a group
+    if (p.P > 1 && sc != p.slice) m_uw = division_magic(uw), m_w = division_magic(ONE ? uw / V : uw);
+    const int rp = divided(TPB, m_nv), t = threadIdx.x;
+    const Lane<V> l(t, nv, m_nv, rp, sc);
     const int64_t r0 = chunk * p.chunk, r1 = min(r0 + p.chunk, p.R);
     const T *base = (const T *)p.x + ((int64_t)img * p.R + r0) * p.ldx + s0;
     const int rows = (int)(r1 - r0);
     for (int u = t; u < nu; u += TPB) piv[u] = to_f32(base[u * uw]);
 
-    float n = 0.f, mean[kVec] = {}, m2[kVec] = {};
+    float n = 0.f, mean[V] = {}, m2[V] = {};
     if (l.live) {
         int r = l.rt;
         const T *q = base + (int64_t)r * p.ldx;
         const int64_t step = (int64_t)rp * p.ldx;
+        Pack<T, V> d[NB], nx[NB];
+        if (r + (NB - 1) * rp < rows)
+#pragma unroll
+            for (int k = 0; k < NB; ++k) d[k] = load_lane<T, V>(q + k * step, l);
         for (; r + (NB - 1) * rp < rows; r += NB * rp) {
-            Pack<T, kVec> d[NB];
-#pragma unroll
-            for (int k = 0; k < NB; ++k) d[k] = load_lane(q + k * step, l);
             q += NB * step;
-            const float f = (float)NB / (n + NB), nf = n * f;
+            if (r + (2 * NB - 1) * rp < rows)
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) {
+                for (int k = 0; k < NB; ++k) nx[k] = load_lane<T, V>(q + k * step, l);
+            const float f = (float)NB * __builtin_amdgcn_rcpf(n + NB), nf = n * f;      // (a weight: its last bit does not matter)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
                 float x[NB], m = 0.f, s = 0.f;
 #pragma unroll
                 for (int k = 0; k < NB; ++k) x[k] = to_f32(d[k].v[j]), m += x[k];
@@ -155,13 +196,15 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
                 m2[j] += fmaf(dm * dm, nf, s);
             }
             n += NB;
+#pragma unroll
+            for (int k = 0; k < NB; ++k) d[k] = nx[k];
         }
         for (; r < rows; r += rp, q += step) {
-            const Pack<T, kVec> d = load_lane(q, l);
-            const float f = 1.f / (n + 1.f), nf = n * f;
+            const Pack<T, V> e = load_lane<T, V>(q, l);
+            const float f = __builtin_amdgcn_rcpf(n + 1.f), nf = n * f;
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const float dm = to_f32(d.v[j]) - mean[j];
+            for (int j = 0; j < V; ++j) {
+                const float dm = to_f32(e.v[j]) - mean[j];
                 mean[j] = fmaf(dm, f, mean[j]);
                 m2[j] = fmaf(dm * dm, nf, m2[j]);
             }
@@ -169,106 +212,110 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
         }
     }
     __syncthreads();             // piv
-    float v[kVec];
-    int un[kVec];
+    float v[V];
+    int un[V];
+    l.template units<ONE>(uw, m_uw, nu, un);
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) un[j] = min((l.lo + j) / uw, nu - 1);
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) v[j] = n * (mean[j] - piv[un[j]]);
-    if (n == 0.f)
-#pragma unroll
-        for (int j = 0; j < kVec; ++j) v[j] = 0.f;
-    unit_sums<TPB, ONE>(v, l, nv, rp, sc, uw, nu, ebuf, tot);
+    for (int j = 0; j < V; ++j) v[j] = n == 0.f ? 0.f : n * (mean[j] - piv[un[j]]);
     const float inv = 1.f / ((float)rows * (float)uw);
+    unit_sums<TPB, V, ONE>(v, l, nv, rp, sc, uw, m_w, nu, ebuf, umean, [&](int u, float s) { return fmaf(s, inv, piv[u]); });
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-        const float d = mean[j] - fmaf(tot[un[j]], inv, piv[un[j]]);
+    for (int j = 0; j < V; ++j) {
+        const float d = mean[j] - umean[un[j]];
         v[j] = n == 0.f ? 0.f : fmaf(n * d, d, m2[j]);
     }
-    float um[(kSliceMax + TPB - 1) / TPB];       // this thread's units' means, before `tot` is written again
-#pragma unroll
-    for (int k = 0; k < (kSliceMax + TPB - 1) / TPB; ++k)
-        if (t + k * TPB < nu) um[k] = fmaf(tot[t + k * TPB], inv, piv[t + k * TPB]);
-    __syncthreads();
-    unit_sums<TPB, ONE>(v, l, nv, rp, sc, uw, nu, ebuf, tot);
+    unit_sums<TPB, V, ONE>(v, l, nv, rp, sc, uw, m_w, nu, ebuf, tot, [](int, float s) { return s; });
     const int U = p.G * p.P, u0 = p.P == 1 ? s0 / p.cg : sl;
     float2 *out = p.part + ((int64_t)img * p.S + chunk) * U + u0;
-#pragma unroll
-    for (int k = 0; k < (kSliceMax + TPB - 1) / TPB; ++k)
-        if (t + k * TPB < nu) out[t + k * TPB] = make_float2(um[k], tot[t + k * TPB]);
+    for (int u = t; u < nu; u += TPB) out[u] = make_float2(umean[u], tot[u]);
 }
 
-// ---- split form, merge: one wave per image and group --------------------------------------------------------------------------------
-__device__ __forceinline__ float wave_sum(float s) {
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-    return s;
-}
-__global__ __launch_bounds__(64) void norm_merge_kernel(NormP p) {
+// ---- split form, merge: a workgroup per image and group joins the chunks and writes (mean, weight / sqrt(var + eps)) of its channels -------
+// The chunks' statistics are read once, all loads on their way together (a chain of dependent reads is what this small kernel would cost).
+__global__ __launch_bounds__(256) void norm_merge_kernel(NormP p) {
+    constexpr int E = 8;                                        // entries per thread in registers: host keeps S * P <= 256 * E
+    __shared__ float red[2][4];
     const int img = blockIdx.x / (unsigned)p.G, g = blockIdx.x - img * p.G, t = threadIdx.x;
-    const int U = p.G * p.P, E = p.S * p.P;
+    const int U = p.G * p.P, n = p.S * p.P;
     const float2 *src = p.part + (int64_t)img * p.S * U + g * p.P;
-    const float pivot = src[0].x;
-    const float inv = 1.f / ((float)p.R * (float)p.cg);
-    auto weight = [&](int c, int k) {
-        const float rows = (float)min(p.chunk, p.R - (int64_t)c * p.chunk);
-        return rows * (float)(p.P == 1 ? p.cg : min(kSliceMax, p.cg - k * kSliceMax));
-    };
-    float s = 0.f;
-    for (int e = t; e < E; e += 64) {
-        const int c = e / p.P, k = e - c * p.P;
-        s += weight(c, k) * (src[(int64_t)c * U + k].x - pivot);
+    const float pivot = src[0].x, inv = 1.f / ((float)p.R * (float)p.cg);
+    float2 v[E];
+    float w[E], s = 0.f;
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int e = t + 256 * k;
+        w[k] = 0.f, v[k] = make_float2(0.f, 0.f);
+        if (e < n) {
+            const int c = p.P == 1 ? e : e / p.P, i = e - c * p.P;
+            v[k] = src[(int64_t)c * U + i];
+            w[k] = (float)min(p.chunk, p.R - (int64_t)c * p.chunk) * (float)(p.P == 1 ? p.cg : min(p.piece, p.cg - i * p.piece));
+        }
     }
-    const float mean = fmaf(wave_sum(s), inv, pivot);
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+        if (w[k] != 0.f) s = fmaf(w[k], v[k].x - pivot, s);
+    s = wave_sum_hi(s);
+    if ((t & 63) == 63) red[0][t >> 6] = s;
+    __syncthreads();
+    const float mean = fmaf((red[0][0] + red[0][1]) + (red[0][2] + red[0][3]), inv, pivot);
     s = 0.f;
-    for (int e = t; e < E; e += 64) {
-        const int c = e / p.P, k = e - c * p.P;
-        const float2 v = src[(int64_t)c * U + k];
-        const float d = v.x - mean;
-        s += fmaf(weight(c, k) * d, d, v.y);
-    }
-    const float var = wave_sum(s) * inv;
-    if (t == 0) p.stat[blockIdx.x] = make_float2(mean, 1.f / sqrtf(var + p.eps));
+#pragma unroll
+    for (int k = 0; k < E; ++k)
+        if (w[k] != 0.f) {
+            const float d = v[k].x - mean;
+            s += fmaf(w[k] * d, d, v[k].y);
+        }
+    s = wave_sum_hi(s);
+    if ((t & 63) == 63) red[1][t >> 6] = s;
+    __syncthreads();
+    const float rstd = 1.f / sqrtf(fmaf((red[1][0] + red[1][1]) + (red[1][2] + red[1][3]), inv, p.eps));
+    float2 *out = p.stat + (int64_t)img * p.C + g * p.cg;
+    const float *wt = p.w ? p.w + g * p.cg : nullptr;
+    for (int c = t; c < p.cg; c += 256) out[c] = make_float2(mean, wt ? rstd * wt[c] : rstd);
 }
 
 // ---- normalise, activate, store: shared by both forms -------------------------------------------------------------------------------
-struct Affine {
-    float mean[kVec], a[kVec], b[kVec];
+template <int V> struct Affine {
+    float mean[V], a[V], b[V];
 };
-__device__ __forceinline__ void finish_row(const float (&x)[kVec], const Affine &f, const NormP &p, float (&y)[kVec]) {
+template <typename T, int V> __device__ __forceinline__ void finish(const Pack<T, V> &d, const Affine<V> &f, const NormP &p, float (&y)[V]) {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) y[j] = apply_act(fmaf(x[j] - f.mean[j], f.a[j], f.b[j]), p.act, p.slope);
+    for (int j = 0; j < V; ++j) y[j] = fmaf(to_f32(d.v[j]) - f.mean[j], f.a[j], f.b[j]);
+    apply_act(y, p.act);
 }
-template <typename T> __device__ __forceinline__ void store_lane(T *row, const Lane &l, const float (&y)[kVec]) {
-    if (l.own == 0 && l.end == kVec) {
-        Pack<T, kVec> r;
+// `whole`: the V channels that were loaded are stored, those of the neighbour with the same values (not where x is written over: this thread
+// may have read them after the neighbour stored)
+template <typename T, int V> __device__ __forceinline__ void store_lane(T *row, const Lane<V> &l, const float (&y)[V], bool whole) {
+    if (l.end == V && (l.own == 0 || whole)) {
+        Pack<T, V> r;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) r.v[j] = from_f32<T>(y[j]);
+        for (int j = 0; j < V; ++j) r.v[j] = from_f32<T>(y[j]);
         store_pack(row + l.lo, r);
         return;
     }
 #pragma unroll
-    for (int j = 0; j < kVec; ++j)
+    for (int j = 0; j < V; ++j)
         if (l.owns(j)) row[l.lo + j] = from_f32<T>(y[j]);
 }
 // 8-bit store of a row's slice (its first column a multiple of 128): 16 consecutive lanes hold one block of 128 columns. `y` of channels that
 // the thread does not own is not looked at; a tail thread's own channels start at `own`, its bytes at column cv * 8.
-__device__ __forceinline__ void store_lane_fp8(uint8_t *qrow, uint8_t *srow, const Lane &l, int sc, bool row_live, const float (&y)[kVec]) {
-    float z[kVec];
-    uint32_t m = 0;
+__device__ __forceinline__ void store_lane_fp8(uint8_t *qrow, uint8_t *srow, const Lane<8> &l, int sc, const float (&y)[8]) {
+    float z[8];
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-        z[j] = 0.f;
-        if (l.own == 0) z[j] = j < l.end ? y[j] : 0.f;
-        else
+    for (int j = 0; j < 8; ++j) z[j] = y[j];
+    if (l.own != 0 || l.end != 8) {                             // own channels to the front, in three steps; zeros behind them
 #pragma unroll
-            for (int i = 0; i < kVec; ++i)
-                if (i == j + l.own) z[j] = y[i];
-        m = max(m, finite_abs_bits(z[j]));
+        for (int b = 1; b < 8; b *= 2)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (l.own & b) z[j] = j + b < 8 ? z[j + b] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j >= l.end - l.own) z[j] = 0.f;
     }
-    const uint32_t byte = fp8_scale_byte(row16_max(m));
+    const uint32_t byte = fp8_scale_byte(row16_finite_max(z));
     const float inv = scale_inverse(byte);
-    if (!row_live) return;
-    const int c0 = l.cv * kVec;
+    const int c0 = l.cv * 8;
     if (c0 < ((sc + 15) & ~15)) {
         uint2 o;
         o.x = to_e4m3x4(z[0] * inv, z[1] * inv, z[2] * inv, z[3] * inv);
@@ -278,26 +325,20 @@ __device__ __forceinline__ void store_lane_fp8(uint8_t *qrow, uint8_t *srow, con
     if ((l.cv & 15) == 0) srow[l.cv >> 4] = (uint8_t)byte;
 }
 
-template <typename T, bool TO8>
-__global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int nsl, int S2, int64_t chunk2) {
-    constexpr int TPB = 256, NB = 4;
+template <typename T, int V, bool TO8>
+__global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int nsl, int S2, int64_t chunk2) {
+    constexpr int TPB = 256, NB = TO8 ? 2 : 4;
     unsigned id = gridDim.x - 1 - blockIdx.x;                  // the opposite order of the first pass
     const int sl = id % (unsigned)nsl;
     id /= (unsigned)nsl;
     const int chunk = id % (unsigned)S2, img = id / (unsigned)S2;
-    const int s0 = sl * kSliceMax, sc = min(kSliceMax, p.C - s0), t = threadIdx.x;
-    const int nv = TO8 ? (sc + kFp8Block - 1) / kFp8Block * (kFp8Block / kVec) : (sc + kVec - 1) / kVec, rp = TPB / nv;
-    const Lane l(t, nv, rp, sc);
+    const int s0 = sl * width, sc = min(width, p.C - s0), t = threadIdx.x;
+    int nv = p.nv;
+    uint32_t m_nv = p.m_nv;
+    if (sc != width) nv = threads_of<V, TO8>(sc), m_nv = division_magic(nv);
+    const int rp = divided(TPB, m_nv);
+    const Lane<V> l(t, nv, m_nv, rp, sc);
     if (!l.live) return;
-    Affine f;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-        const int c = s0 + min(l.lo + j, sc - 1);
-        const float2 st = p.stat[img * p.G + c / p.cg];
-        f.mean[j] = st.x;
-        f.a[j] = p.w ? st.y * p.w[c] : st.y;
-        f.b[j] = p.b ? p.b[c] : 0.f;
-    }
     const int64_t r0 = chunk * chunk2;
     const int rows = (int)(min(r0 + chunk2, p.R) - r0);
     const int64_t at = (int64_t)img * p.R + r0 + l.rt;
@@ -305,195 +346,232 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int nsl, int S
     T *o = TO8 ? nullptr : (T *)p.y + at * p.ldy + s0;
     uint8_t *oq = TO8 ? p.q + at * p.ldq + s0 : nullptr, *os = TO8 ? p.qs + at * p.ldqs + s0 / kFp8Block : nullptr;
     const int64_t sx = (int64_t)rp * p.ldx;
-    auto emit = [&](const Pack<T, kVec> &d, int64_t k) {
-        float x[kVec], y[kVec];
+    Affine<V> f;
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) x[j] = to_f32(d.v[j]);
-        finish_row(x, f, p, y);
-        if constexpr (TO8) store_lane_fp8(oq + k * rp * p.ldq, os + k * rp * p.ldqs, l, sc, true, y);
-        else store_lane(o + k * rp * p.ldy, l, y);
+    for (int j = 0; j < V; ++j) {
+        const int c = s0 + min(l.lo + j, sc - 1);
+        const float2 st = p.stat[(int64_t)img * p.C + c];
+        f.mean[j] = st.x, f.a[j] = st.y;
+        f.b[j] = p.b ? p.b[c] : 0.f;
+    }
+    auto emit = [&](const Pack<T, V> &d, int64_t k) {
+        float y[V];
+        finish<T, V>(d, f, p, y);
+        if constexpr (TO8) store_lane_fp8(oq + k * rp * p.ldq, os + k * rp * p.ldqs, l, sc, y);
+        else store_lane<T, V>(o + k * rp * p.ldy, l, y, !p.in_place);
     };
     int r = l.rt;
     int64_t k = 0;
     // (lanes of a row of 16 share rt: they enter and leave these loops together, so the block maximum sees all of them)
     for (; r + (NB - 1) * rp < rows; r += NB * rp, k += NB) {
-        Pack<T, kVec> d[NB];
+        Pack<T, V> d[NB];
 #pragma unroll
-        for (int i = 0; i < NB; ++i) d[i] = load_lane(q + (k + i) * sx, l);
+        for (int i = 0; i < NB; ++i) d[i] = load_lane<T, V, TO8>(q + (k + i) * sx, l);
 #pragma unroll
         for (int i = 0; i < NB; ++i) emit(d[i], k + i);
     }
-    for (; r < rows; r += rp, ++k) emit(load_lane(q + k * sx, l), k);
+    for (; r < rows; r += rp, ++k) emit(load_lane<T, V, TO8>(q + k * sx, l), k);
 }
 
 // ---- resident form --------------------------------------------------------------------------------------------------------------------
-template <typename T, int TPB, int NIT, bool ONE, bool TO8>
+// Rolled loops on purpose: the form serves small maps, whose time is latency, and 50 KB of straight-line code cost more to fetch than the map
+// (27 us for 3 x 1961 x 100 fp16 with the slice in registers and everything unrolled).
+template <typename T, int V, int TPB, bool ONE, bool TO8>
 __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
-    __shared__ float ebuf[TPB * kVec];
-    extern __shared__ float dyn[];                             // tot[units of the slice], piv[...]
+    constexpr int NB = 4;
+    using D = Pack<T, V>;
+    using W = std::conditional_t<(sizeof(D) >= 16), i32x4, T>;  // how a thread's data lies in the LDS
+    extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
     const int sl = blockIdx.x % (unsigned)p.nslices, img = blockIdx.x / (unsigned)p.nslices, t = threadIdx.x;
-    const int s0 = sl * p.slice, sc = min(p.slice, p.C - s0), uw = p.cg, nu = sc / uw;
-    float *tot = dyn, *piv = dyn + p.slice / p.cg;
-    const int nv = TO8 ? (sc + kFp8Block - 1) / kFp8Block * (kFp8Block / kVec) : (sc + kVec - 1) / kVec, rp = TPB / nv;
-    const Lane l(t, nv, rp, sc);
-    const T *base = (const T *)p.x + (int64_t)img * p.R * p.ldx + s0;
+    const int s0 = sl * p.slice, sc = min(p.slice, p.C - s0), uw = p.cg, mu = divided(p.slice, p.m_uw), nu = divided(sc, p.m_uw);
+    float *ebuf = (float *)dyn, *umean = ebuf + TPB * (ONE ? 1 : V), *urstd = umean + mu, *piv = urstd + mu;
+    constexpr int Q = sizeof(D) / sizeof(W);
+    W *data = (W *)(dyn + (4 * (TPB * (ONE ? 1 : V) + 3 * mu) + 15) / 16 * 16) + t;
+    auto put = [&](W *to, const D &x) {
+        W v[Q];
+        __builtin_memcpy(v, &x, sizeof(x));
+#pragma unroll
+        for (int i = 0; i < Q; ++i) to[i * TPB] = v[i];
+    };
+    auto get = [&](const W *from) {
+        W v[Q];
+#pragma unroll
+        for (int i = 0; i < Q; ++i) v[i] = from[i * TPB];
+        D x;
+        __builtin_memcpy(&x, v, sizeof(x));
+        return x;
+    };
+    int nv = p.nv;
+    uint32_t m_nv = p.m_nv;
+    if (sc != p.slice) nv = threads_of<V, TO8>(sc), m_nv = division_magic(nv);
+    const int rp = divided(TPB, m_nv);
+    const Lane<V> l(t, nv, m_nv, rp, sc);
     const int R = (int)p.R;
-    Pack<T, kVec> d[NIT];
+    const T *base = (const T *)p.x + (int64_t)img * R * p.ldx + s0;
+    D d[NB];
+    auto load = [&](int r) {
 #pragma unroll
-    for (int k = 0; k < NIT; ++k) {
-        const int r = l.rt + k * rp;
-        d[k] = load_lane(base + (int64_t)min(r, R - 1) * p.ldx, l);
-    }
+        for (int k = 0; k < NB; ++k) d[k] = load_lane<T, V, TO8>(base + (int64_t)min(r + k * rp, R - 1) * p.ldx, l);
+    };
+    load(l.rt);
     for (int u = t; u < nu; u += TPB) piv[u] = to_f32(base[u * uw]);
-    __syncthreads();
-    int un[kVec];
-    float pv[kVec], v[kVec] = {};
+    Affine<V> f;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) un[j] = min((l.lo + j) / uw, nu - 1), pv[j] = piv[un[j]];
-#pragma unroll
-    for (int k = 0; k < NIT; ++k)
-        if (l.rt + k * rp < R)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) v[j] += to_f32(d[k].v[j]) - pv[j];
-    const float inv = 1.f / ((float)R * (float)uw);
-    const int ev = (sc + kVec - 1) / kVec;
-    Lane le = l;                                               // (the 8-bit form's padding lanes own nothing and take no part in the sums)
-    le.live = l.live && l.cv < ev;
-    unit_sums<TPB, ONE>(v, le, nv, rp, sc, uw, nu, ebuf, tot);
-    Affine f;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) f.mean[j] = fmaf(tot[un[j]], inv, pv[j]), v[j] = 0.f;
-#pragma unroll
-    for (int k = 0; k < NIT; ++k)
-        if (l.rt + k * rp < R)
-#pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const float x = to_f32(d[k].v[j]) - f.mean[j];
-                v[j] = fmaf(x, x, v[j]);
-            }
-    __syncthreads();                                           // every thread has its means
-    unit_sums<TPB, ONE>(v, le, nv, rp, sc, uw, nu, ebuf, tot);
-    if (!l.live) return;
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
+    for (int j = 0; j < V; ++j) {
         const int c = s0 + min(l.lo + j, sc - 1);
-        const float rstd = 1.f / sqrtf(fmaf(tot[un[j]], inv, p.eps));
-        f.a[j] = p.w ? rstd * p.w[c] : rstd;
+        f.a[j] = p.w ? p.w[c] : 1.f;
         f.b[j] = p.b ? p.b[c] : 0.f;
     }
+    int un[V];
+    l.template units<ONE>(uw, p.m_uw, nu, un);
+    __syncthreads();
+    float v[V] = {};
 #pragma unroll
-    for (int k = 0; k < NIT; ++k) {
-        const int r = l.rt + k * rp;
-        if (r >= R) break;
-        float x[kVec], y[kVec];
+    for (int j = 0; j < V; ++j) f.mean[j] = piv[un[j]];
+    W *at = data;
+    for (int r = l.rt; r < R;) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) x[j] = to_f32(d[k].v[j]);
-        finish_row(x, f, p, y);
-        const int64_t at = (int64_t)img * p.R + r;
-        if constexpr (TO8) store_lane_fp8(p.q + at * p.ldq + s0, p.qs + at * p.ldqs + s0 / kFp8Block, l, sc, true, y);
-        else store_lane((T *)p.y + at * p.ldy + s0, l, y);
+        for (int k = 0; k < NB; ++k) {
+            put(at + k * Q * TPB, d[k]);
+            const bool on = r + k * rp < R;
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] += on ? to_f32(d[k].v[j]) - f.mean[j] : 0.f;
+        }
+        at += NB * Q * TPB;
+        r += NB * rp;
+        if (r < R) load(r);
+    }
+    const float inv = 1.f / ((float)R * (float)uw);
+    Lane<V> le = l;                                            // (the 8-bit form's padding lanes own nothing and take no part in the sums)
+    le.live = l.live && l.cv * V < sc;
+    unit_sums<TPB, V, ONE>(v, le, nv, rp, sc, uw, p.m_w, nu, ebuf, umean, [&](int u, float s) { return fmaf(s, inv, piv[u]); });
+#pragma unroll
+    for (int j = 0; j < V; ++j) f.mean[j] = umean[un[j]], v[j] = 0.f;
+    at = data;
+    for (int r = l.rt; r < R; r += rp, at += Q * TPB) {
+        const D x = get(at);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float e = to_f32(x.v[j]) - f.mean[j];
+            v[j] = fmaf(e, e, v[j]);
+        }
+    }
+    unit_sums<TPB, V, ONE>(v, le, nv, rp, sc, uw, p.m_w, nu, ebuf, urstd, [&](int, float s) { return 1.f / sqrtf(fmaf(s, inv, p.eps)); });
+    if (!l.live) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) f.a[j] *= urstd[un[j]];
+    at = data;
+    int64_t row = (int64_t)img * R + l.rt;
+    for (int r = l.rt; r < R; r += rp, at += Q * TPB, row += rp) {     // (the 16 lanes of a block share r)
+        float y[V];
+        finish<T, V>(get(at), f, p, y);
+        if constexpr (TO8) store_lane_fp8(p.q + row * p.ldq + s0, p.qs + row * p.ldqs + s0 / kFp8Block, l, sc, y);
+        else store_lane<T, V>((T *)p.y + row * p.ldy + s0, l, y, true);
     }
 }
 
 // ---- which form, with which split ---------------------------------------------------------------------------------------------------
 struct NormPlan {
     bool resident;
-    int tpb, nit;            // resident
-    int slice, nslices, P, S;
+    int tpb;                 // resident
+    size_t lds;
+    int V;
+    int slice, nslices, P, piece, S;
     int64_t chunk;
     bool one;
 };
 static int gcd_i(int a, int b) { return b ? gcd_i(b, a % b) : a; }
+constexpr int kMergeMax = 2048;          // chunks x pieces that the merge holds in registers
+constexpr int kResidentBytes = 128 * 1024;
 
 static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8) {
     NormPlan q{};
     const int cg = C / G;
-    // resident: the narrowest slice of whole groups whose rows are 64 contiguous bytes (a slice of 8-bit rows starts at a block: a multiple
-    // of 128 columns, or the whole row), if 1024 threads can hold it: 64 VGPRs of data each
-    int64_t unit = to8 ? (int64_t)cg / gcd_i(cg, kFp8Block) * kFp8Block : cg;
-    int64_t slice = unit * ((64 / es + unit - 1) / unit);
+    int V = to8 ? 8 : 16 / es;
+    // Resident: the narrowest slice of whole groups whose rows are 32 contiguous bytes (a slice of 8-bit rows starts at a block: a multiple
+    // of 128 columns, or the whole row), if the LDS holds it
+    const int64_t unit = to8 ? (int64_t)cg / gcd_i(cg, kFp8Block) * kFp8Block : cg;
+    int64_t slice = unit * ((32 / es + unit - 1) / unit);
     if (slice > C) slice = C;
-    const int maxit = es == 4 ? 8 : 16;
-    const int64_t nv = to8 ? (slice + kFp8Block - 1) / kFp8Block * (kFp8Block / kVec) : (slice + kVec - 1) / kVec;
-    if (nv <= 1024 && R <= (int64_t)maxit * (1024 / nv)) {
-        q.resident = true;
+    const auto last = [&](int64_t w) { return C % w ? C % w : w; };
+    if (!to8 && last(slice) < V) V = 1;
+    q.V = V;
+    q.one = cg % V == 0;
+    const int64_t nv = to8 ? (slice + kFp8Block - 1) / kFp8Block * (kFp8Block / 8) : (slice + V - 1) / V;
+    if (nv <= 512 && R <= kResidentBytes) {
+        q.tpb = nv <= 256 && R <= 8 * (256 / nv) ? 256 : 512;
+        const int64_t rp = q.tpb / nv, its = (R + 4 * rp - 1) / (4 * rp) * 4;
         q.slice = (int)slice;
-        q.nslices = (int)((C + slice - 1) / slice);
-        q.tpb = nv <= 256 && R <= 4 * (256 / nv) ? 256 : 1024;
-        const int64_t rp = q.tpb / nv, need = (R + rp - 1) / rp;
-        q.nit = 1;
-        while (q.nit < need) q.nit *= 2;
-        q.one = cg % kVec == 0;
-        return q;
+        q.lds = (4 * (size_t)(q.tpb * (q.one ? 1 : V) + 3 * (slice / cg)) + 15) / 16 * 16 + (size_t)(its * q.tpb * V * es);
+        if (q.lds <= kResidentBytes + 16 * 1024) {
+            q.resident = true;
+            q.nslices = (int)((C + slice - 1) / slice);
+            return q;
+        }
     }
-    q.P = cg > kSliceMax ? (cg + kSliceMax - 1) / kSliceMax : 1;
-    q.slice = q.P == 1 ? kSliceMax / cg * cg : kSliceMax;
-    if (q.P == 1 && q.slice > C) q.slice = C;
-    q.nslices = q.P == 1 ? (C + q.slice - 1) / q.slice : G * q.P;
-    q.one = cg % kVec == 0;
+    for (V = 16 / es, q.piece = kSliceMax;; V = 1, q.piece = 256) {
+        q.P = (cg + q.piece - 1) / q.piece;
+        q.slice = q.P == 1 ? std::min(q.piece / cg * cg, C) : q.piece;
+        q.nslices = q.P == 1 ? (C + q.slice - 1) / q.slice : G * q.P;
+        if (V == 1 || (q.P == 1 ? last(q.slice) : (cg - 1) % q.piece + 1) >= V) break;
+    }
+    q.V = V;
+    q.one = cg % V == 0;
     // about 4 workgroups per CU, each with at least 8 rows per thread
-    const int64_t rp = 256 / ((std::min(q.slice, C) + kVec - 1) / kVec);
-    int64_t S = 1024 / ((int64_t)images * q.nslices);
-    if (S < 1) S = 1;
+    const int64_t rp = 256 / ((q.slice + V - 1) / V);
+    int64_t S = std::min<int64_t>(1024 / std::max<int64_t>(1, std::min<int64_t>((int64_t)images * q.nslices, 1024)), std::max(1, kMergeMax / q.P));
     int64_t chunk = (R + S - 1) / S;
     if (chunk < 8 * rp) chunk = 8 * rp;
-    if (chunk > 0x40000000) chunk = 0x40000000;
     q.chunk = chunk;
     q.S = (int)((R + chunk - 1) / chunk);
     return q;
 }
 
-static int64_t norm_ws(const NormPlan &q, int images, int G) {
-    return q.resident ? 0 : 8 * ((int64_t)images * q.S * G * q.P + (int64_t)images * G);
+static int64_t norm_ws(const NormPlan &q, int images, int C, int G) {
+    return q.resident ? 0 : 8 * ((int64_t)images * q.S * G * q.P + (int64_t)images * C);
 }
 
-template <typename T, int TPB, int NIT>
-static void launch_resident(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {
-    const unsigned grid = (unsigned)(images * q.nslices);
-    const size_t dyn = 8 * (size_t)(q.slice / p.cg);
-    if (to8) {
-        if (q.one) norm_resident_kernel<T, TPB, NIT, true, true><<<grid, TPB, dyn, s>>>(p);
-        else norm_resident_kernel<T, TPB, NIT, false, true><<<grid, TPB, dyn, s>>>(p);
-    } else {
-        if (q.one) norm_resident_kernel<T, TPB, NIT, true, false><<<grid, TPB, dyn, s>>>(p);
-        else norm_resident_kernel<T, TPB, NIT, false, false><<<grid, TPB, dyn, s>>>(p);
-    }
+template <typename T, int V, int TPB, bool ONE, bool TO8> static int launch_resident(const NormP &p, const NormPlan &q, int images, hipStream_t s) {
+    static LdsGrant grant;
+    if (int rc = grant.ensure((const void *)norm_resident_kernel<T, V, TPB, ONE, TO8>, q.lds, 64 * 1024)) return rc;
+    NormP n = p;
+    n.nv = threads_of<V, TO8>(q.slice), n.m_nv = division_magic(n.nv);
+    n.m_uw = division_magic(p.cg), n.m_w = division_magic(ONE ? p.cg / V : p.cg);
+    norm_resident_kernel<T, V, TPB, ONE, TO8><<<(unsigned)(images * q.nslices), TPB, q.lds, s>>>(n);
+    return launch_status("group_norm");
+}
+template <typename T, int TPB> static int launch_resident(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {
+    if (to8) return q.one ? launch_resident<T, 8, TPB, true, true>(p, q, images, s) : launch_resident<T, 8, TPB, false, true>(p, q, images, s);
+    if (q.V == 1) return launch_resident<T, 1, TPB, true, false>(p, q, images, s);
+    return q.one ? launch_resident<T, kVecOf<T>, TPB, true, false>(p, q, images, s) : launch_resident<T, kVecOf<T>, TPB, false, false>(p, q, images, s);
 }
 
 template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {
-    if (q.resident) {
-        if (q.tpb == 256) switch (q.nit) {
-            case 1: launch_resident<T, 256, 1>(p, q, images, to8, s); break;
-            case 2: launch_resident<T, 256, 2>(p, q, images, to8, s); break;
-            default: launch_resident<T, 256, 4>(p, q, images, to8, s); break;
-        } else switch (q.nit) {
-            case 1: launch_resident<T, 1024, 1>(p, q, images, to8, s); break;
-            case 2: launch_resident<T, 1024, 2>(p, q, images, to8, s); break;
-            case 4: launch_resident<T, 1024, 4>(p, q, images, to8, s); break;
-            case 8: launch_resident<T, 1024, 8>(p, q, images, to8, s); break;
-            default:
-                if constexpr (sizeof(T) == 2) launch_resident<T, 1024, 16>(p, q, images, to8, s);
-                break;
-        }
-        return launch_status("group_norm");
-    }
+    if (q.resident) return q.tpb == 256 ? launch_resident<T, 256>(p, q, images, to8, s) : launch_resident<T, 512>(p, q, images, to8, s);
+    constexpr int V = kVecOf<T>;
     const unsigned g1 = (unsigned)((int64_t)images * q.S * q.nslices);
-    if (q.one) norm_stats_kernel<T, true><<<g1, 256, 0, s>>>(p);
-    else norm_stats_kernel<T, false><<<g1, 256, 0, s>>>(p);
-    norm_merge_kernel<<<(unsigned)(images * p.G), 64, 0, s>>>(p);
-    const int nsl = (p.C + kSliceMax - 1) / kSliceMax;
-    const int sc = std::min(p.C, kSliceMax);
-    const int nv = to8 ? (sc + kFp8Block - 1) / kFp8Block * (kFp8Block / kVec) : (sc + kVec - 1) / kVec;
+    NormP n = p;
+    const int uw = q.P == 1 ? p.cg : q.piece;
+    n.nv = q.V == 1 ? q.slice : threads_of<V, false>(q.slice), n.m_nv = division_magic(n.nv);
+    n.m_uw = division_magic(uw), n.m_w = division_magic(q.one ? uw / q.V : uw);
+    if (q.V == 1) norm_stats_kernel<T, 1, true><<<g1, 256, 0, s>>>(n);
+    else if (q.one) norm_stats_kernel<T, V, true><<<g1, 256, 0, s>>>(n);
+    else norm_stats_kernel<T, V, false><<<g1, 256, 0, s>>>(n);
+    norm_merge_kernel<<<(unsigned)(images * p.G), 256, 0, s>>>(p);
+    // the normalising pass: slices of columns that need not hold whole groups
+    const int tail = p.C % kSliceMax, V2 = to8 ? 8 : tail && tail < V ? 1 : V, width = V2 == 1 ? 256 : kSliceMax;
+    const int nsl = (p.C + width - 1) / width, sc = std::min(p.C, width);
+    const int nv = to8 ? threads_of<8, true>(sc) : (sc + V2 - 1) / V2;
     const int64_t rp = 256 / nv;
-    int64_t S2 = 4096 / ((int64_t)images * nsl);
-    if (S2 < 1) S2 = 1;
+    n.nv = nv, n.m_nv = division_magic(nv);
+    int64_t S2 = std::max<int64_t>(1, 4096 / std::max<int64_t>(1, (int64_t)images * nsl));
     int64_t chunk2 = (p.R + S2 - 1) / S2;
     if (chunk2 < 4 * rp) chunk2 = 4 * rp;
-    if (chunk2 > 0x40000000) chunk2 = 0x40000000;
     S2 = (p.R + chunk2 - 1) / chunk2;
     const unsigned g2 = (unsigned)((int64_t)images * S2 * nsl);
-    if (to8) norm_apply_kernel<T, true><<<g2, 256, 0, s>>>(p, nsl, (int)S2, chunk2);
-    else norm_apply_kernel<T, false><<<g2, 256, 0, s>>>(p, nsl, (int)S2, chunk2);
+    if (to8) norm_apply_kernel<T, 8, true><<<g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2);
+    else if (V2 == 1) norm_apply_kernel<T, 1, false><<<g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2);
+    else norm_apply_kernel<T, V, false><<<g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2);
     return launch_status("group_norm");
 }
 
@@ -520,7 +598,7 @@ using namespace lssvc;
 
 extern "C" int64_t lssvc_group_norm_workspace_bytes(int64_t rows, int32_t images, int32_t cols, int32_t groups, int32_t dtype, int32_t to_fp8) {
     if (rows <= 0 || images <= 0 || cols <= 0 || groups <= 0 || cols % groups || rows % images || !rows_type_ok(dtype)) return 0;
-    return norm_ws(norm_plan(rows / images, images, cols, groups, rows_type_size(dtype), to_fp8 != 0), images, groups);
+    return norm_ws(norm_plan(rows / images, images, cols, groups, rows_type_size(dtype), to_fp8 != 0), images, cols, groups);
 }
 
 extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t groups, const float *weight, const float *bias, float eps,
@@ -542,8 +620,9 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     const int64_t R = x->rows / images;
     const int es = rows_type_size(x->dtype);
     const NormPlan q = norm_plan(R, images, x->cols, groups, es, y8 != nullptr);
-    const int64_t need = norm_ws(q, images, groups);
+    const int64_t need = norm_ws(q, images, x->cols, groups);
     LSSVC_CHECK(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), "group_norm: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need, (long long)workspace_bytes);
+    LSSVC_CHECK(R <= (1LL << 30) && q.P <= kMergeMax, "group_norm: an image of %lld rows x %d channels in %d groups is too large", (long long)R, x->cols, groups);
     LSSVC_CHECK((int64_t)images * std::max<int64_t>(groups, (int64_t)q.nslices * std::max(q.S, 1)) < (1LL << 31), "group_norm: too many images or groups for one launch");
     NormP p{};
     p.x = x->ptr;
@@ -553,10 +632,11 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     p.R = R;
     p.w = weight, p.b = bias;
     p.C = x->cols, p.G = groups, p.cg = x->cols / groups;
-    p.S = q.S, p.P = q.P, p.chunk = q.chunk, p.slice = q.slice, p.nslices = q.nslices;
-    p.act = act, p.eps = eps, p.slope = slope;
+    p.S = q.S, p.P = q.P, p.piece = q.piece, p.chunk = q.chunk, p.slice = q.slice, p.nslices = q.nslices;
+    p.act = make_act(act, slope), p.eps = eps;
+    p.in_place = y && y->ptr == x->ptr;
     p.stat = (float2 *)workspace;
-    p.part = p.stat + (int64_t)images * groups;
+    p.part = p.stat + (int64_t)images * x->cols;
     hipStream_t s = (hipStream_t)stream;
     if (x->dtype == LSSVC_F32) return launch_norm<float>(p, q, images, y8 != nullptr, s);
     if (x->dtype == LSSVC_F16) return launch_norm<f16_t>(p, q, images, y8 != nullptr, s);

@@ -26,12 +26,6 @@ template <typename T> __device__ __forceinline__ void load8(const T *row, int c,
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = c + j < cols ? to_f32(row[c + j]) : 0.f;
 }
-__device__ __forceinline__ uint32_t max8(const float (&v)[8]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, finite_abs_bits(v[j]));
-    return m;
-}
 __device__ __forceinline__ void store8(uint8_t *q, const float (&v)[8], float inv) {
     uint2 o;
     o.x = to_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
@@ -48,38 +42,37 @@ template <typename T> __global__ __launch_bounds__(256) void quant_rows_kernel(Q
     const int k = (int)(b - r * p.kb), c = k * kFp8Block + (threadIdx.x & 15) * 8;
     float v[8];
     load8((const T *)p.x + r * p.ldx, c, p.cols, v);
-    const uint32_t byte = fp8_scale_byte(row16_max(max8(v)));
+    const uint32_t byte = fp8_scale_byte(row16_finite_max(v));
     if (c < ((p.cols + 15) & ~15)) store8(p.q + r * p.ldq + c, v, scale_inverse(byte));
     if ((threadIdx.x & 15) == 0) p.s[r * p.lds + k] = (uint8_t)byte;
 }
 
-// 128 x 128 blocks: a workgroup holds one, 8 rows of 8 columns per thread
-template <typename T> __global__ __launch_bounds__(256) void quant_tiles_kernel(QuantP p) {
-    __shared__ uint32_t wmax[4];
+// 128 x 128 blocks: a workgroup holds one, 4 rows of 8 columns per thread
+template <typename T> __global__ __launch_bounds__(512) void quant_tiles_kernel(QuantP p) {
+    __shared__ uint32_t wmax[32];
     const int64_t rb = blockIdx.x / (unsigned)p.kb;
     const int k = (int)(blockIdx.x - rb * p.kb), t = threadIdx.x;
     const int c = k * kFp8Block + (t & 15) * 8;
     const int64_t r0 = rb * kFp8Block + (t >> 4);
-    float v[8][8];
+    float v[4][8];
     uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int64_t r = r0 + 16 * i;
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + 32 * i;
         if (r < p.rows) load8((const T *)p.x + r * p.ldx, c, p.cols, v[i]);
         else
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-        m = max(m, max8(v[i]));
+        m = max(m, row16_finite_max(v[i]));
     }
-    for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o));
-    if ((t & 63) == 0) wmax[t >> 6] = m;
+    if ((t & 15) == 0) wmax[t >> 4] = m;
     __syncthreads();
-    m = max(max(wmax[0], wmax[1]), max(wmax[2], wmax[3]));
+    m = row16_max(max(wmax[t & 15], wmax[16 + (t & 15)]));
     const uint32_t byte = fp8_scale_byte(m);
     const float inv = scale_inverse(byte);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int64_t r = r0 + 16 * i;
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + 32 * i;
         if (r < p.rows && c < ((p.cols + 15) & ~15)) store8(p.q + r * p.ldq + c, v[i], inv);
     }
     if (t == 0) p.s[rb * p.lds + k] = (uint8_t)byte;
@@ -93,7 +86,7 @@ template <typename T> static int launch_quant(const QuantP &p, int block_rows, h
     } else {
         const int64_t tiles = (p.rows + kFp8Block - 1) / kFp8Block * p.kb;
         LSSVC_CHECK(tiles < (1LL << 31), "quantize_fp8: %lld blocks do not fit one launch", (long long)tiles);
-        quant_tiles_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(p);
+        quant_tiles_kernel<T><<<(unsigned)tiles, 512, 0, s>>>(p);
     }
     return launch_status("quantize_fp8");
 }

@@ -53,12 +53,26 @@ template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(con
 }
 template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) { __builtin_memcpy(p, &r, sizeof(r)); }
 
-// exp and reciprocal at the hardware's 1 ulp: 2^-22 relative beside the 2^-24 .. 2^-8 of the stored result. NaN passes through all.
-__device__ __forceinline__ float apply_act(float v, int act, float slope) {
-    if (act == LSSVC_ACT_NONE) return v;
-    if (act == LSSVC_ACT_LRELU) return v >= 0.f ? v : v * slope;
-    if (act == LSSVC_ACT_RELU) return v < 0.f ? 0.f : v;
-    return v * __builtin_amdgcn_rcpf(1.f + __expf(-v));
+// Activations, for N values at a time so that the choice is made once. None, relu and lrelu are one form, v < 0 ? max(v, floor) * slope : v, with
+// slope 1, 0 or the caller's (floor keeps relu's -inf * 0 from being NaN). silu: exp and reciprocal at the hardware's 1 ulp, 2^-22 relative
+// beside the 2^-24 .. 2^-8 of the stored result. NaN passes through.
+struct Act {
+    float slope, floor;
+    int silu;
+};
+inline Act make_act(int act, float slope) {
+    const float inf = __builtin_inff();
+    if (act == LSSVC_ACT_SILU) return Act{0.f, 0.f, 1};
+    return act == LSSVC_ACT_NONE ? Act{1.f, -inf, 0} : act == LSSVC_ACT_RELU ? Act{0.f, -3.402823466e38f, 0} : Act{slope, -inf, 0};
+}
+template <int N> __device__ __forceinline__ void apply_act(float (&v)[N], const Act &a) {
+    if (a.silu) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] * __builtin_amdgcn_rcpf(1.f + __expf(-v[i]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? fmaxf(v[i], a.floor) * a.slope : v[i];
+    }
 }
 
 // ---- 8-bit blocks ---------------------------------------------------------------------------------------------------------------
@@ -69,11 +83,40 @@ __device__ __forceinline__ uint32_t row16_max(uint32_t v) {
     v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x122, 0xf, 0xf, true));
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x121, 0xf, 0xf, true));
 }
-// |x| as an ordered integer; what is not finite counts as 0 and does not move a scale
-__device__ __forceinline__ uint32_t finite_abs_bits(float x) {
-    const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-    return b < 0x7f800000u ? b : 0u;
+// The largest |x| among 8 values per lane of the finite ones, over the 16 lanes of a DPP row, as ordered bits. The plain maximum first: only
+// where it is not finite are such values left out one by one.
+__device__ __forceinline__ uint32_t row16_finite_max(const float (&z)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(z[j]) & 0x7fffffffu);
+    m = row16_max(m);
+    if (m >= 0x7f800000u) {                  // (the 16 lanes agree)
+        m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t b = __float_as_uint(z[j]) & 0x7fffffffu;
+            m = max(m, b < 0x7f800000u ? b : 0u);
+        }
+        m = row16_max(m);
+    }
+    return m;
 }
+// sum over the wave in a fixed order, valid in lane 63
+__device__ __forceinline__ float wave_sum_hi(float v) {
+#define LSSVC_DPP_ADD(ctrl, rows) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, rows, 0xf, false))
+    LSSVC_DPP_ADD(0x111, 0xf);               // row_shr:1, 2, 4, 8: lane 15 of each row has the row's sum
+    LSSVC_DPP_ADD(0x112, 0xf);
+    LSSVC_DPP_ADD(0x114, 0xf);
+    LSSVC_DPP_ADD(0x118, 0xf);
+    LSSVC_DPP_ADD(0x142, 0xa);               // row_bcast:15 into rows 1 and 3
+    LSSVC_DPP_ADD(0x143, 0xc);               // row_bcast:31 into rows 2 and 3
+#undef LSSVC_DPP_ADD
+    return v;
+}
+// t / n for t < 2^16 and n < 2^16: one multiplication; magic = division_magic(n)
+__host__ __device__ __forceinline__ uint32_t division_magic(uint32_t n) { return n > 1 ? 0xffffffffu / n + 1 : 0; }
+__device__ __forceinline__ int divided(int t, uint32_t magic) { return magic ? (int)__umulhi((uint32_t)t, magic) : t; }
+
 // The exponent byte of the smallest power of two s >= 2^-126 with amax <= 448 s (1 where amax = 0). amax = m 2^k with m in [0.5, 1)
 // and 448 = 0.875 * 2^9, so s = 2^(k - 9) where m <= 0.875 and 2^(k - 8) otherwise; k = field - 126.
 __device__ __forceinline__ uint32_t fp8_scale_byte(uint32_t amax_bits) {

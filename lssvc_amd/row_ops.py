@@ -14,8 +14,6 @@ Rows are given as one of
 and come back as the same kind. Everything is enqueued on the current stream of the tensors' device; nothing synchronises. The
 operators are forward operators (a tensor that requires a gradient is refused) and are not part of compiled frame plans.
 """
-import ctypes as C
-
 import torch
 
 from . import _lib, hip_ops
@@ -69,8 +67,6 @@ def _rows(x, name):
 
 
 def _vector(x, name, n, device):
-    if x is None:
-        return None
     if not (isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.dim() == 1 and x.shape[0] == n and (n == 1 or x.stride(0) == 1) and x.device == device):
         _refuse("row_ops: %s has to be %d adjacent fp32 values on %s", name, n, device)
     _no_grad(x, name)
@@ -84,23 +80,14 @@ def _act_code(act):
     return code
 
 
-class _On:
-    """The launch context of one call: the tensors' device is made current if it is not."""
-    __slots__ = ("guard",)
+_raw_stream = torch._C._cuda_getCurrentRawStream     # torch.cuda.current_stream(device).cuda_stream without the Stream object (1 us a call)
 
-    def __init__(self, device):
-        if hip_ops.PLAN_RECORDER is not None:
-            _refuse("row_ops: not part of compiled frame plans")
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _elsewhere(device):
+    """Whether `device` has to be made current for a call (every entry point does that around itself)."""
+    if hip_ops.PLAN_RECORDER is not None:
+        _refuse("row_ops: not part of compiled frame plans")
+    return device.index != torch.cuda.current_device()
 
 
 def _same_device(device, **others):
@@ -118,7 +105,7 @@ class Fp8Rows:
 
     Tensors that the kernels can read as they are stay where they are; others (columns that are no multiple of 16, odd pitches or
     bases) are copied once, here, into rows with zeros behind the last column."""
-    __slots__ = ("values", "scale", "rows", "cols", "block_rows", "_c", "_keep")
+    __slots__ = ("_values", "_scale", "_store", "rows", "cols", "block_rows", "device", "_c")
 
     def __init__(self, values, scale, block_rows=1):
         if not isinstance(values, torch.Tensor) or values.dtype != _E4M3 or values.dim() != 2 or not values.is_cuda:
@@ -144,28 +131,41 @@ class Fp8Rows:
     def _set(self, values, scale, block_rows):
         rows, cols = values.shape
         kb = -(-cols // BLOCK)
-        self.values, self.scale, self.rows, self.cols, self.block_rows = values, scale, rows, cols, block_rows
+        self._values, self._scale, self.rows, self.cols, self.block_rows, self.device = values, scale, rows, cols, block_rows, values.device
         e8m0 = scale.dtype == _E8M0
         ld = values.stride(0) if rows > 1 else -(-cols // 16) * 16
         sld = scale.stride(0) if scale.shape[0] > 1 else (-(-kb // 4) * 4 if e8m0 else kb)
         self._c = Fp8(values.data_ptr(), scale.data_ptr(), rows, ld, sld, cols, block_rows, 1 if e8m0 else 0, 0)
+        self._store = None
+
+    # values and scale of operands that the kernels made live in one buffer and become tensors when somebody looks
+    @property
+    def values(self):
+        if self._values is None:
+            self._values = self._store.view(_E4M3).as_strided((self.rows, self.cols), (self._c.ld, 1))
+        return self._values
 
     @property
-    def device(self):
-        return self.values.device
+    def scale(self):
+        if self._scale is None:
+            self._scale = self._store.view(_E8M0).as_strided((-(-self.rows // self.block_rows), -(-self.cols // BLOCK)), (self._c.scale_ld, 1), self.rows * self._c.ld)
+        return self._scale
 
     @staticmethod
     def empty(rows, cols, device, block_rows=1):
         """Uninitialised rows with e8m0 scales, for `out=` of the operators that write 8-bit rows."""
-        if block_rows not in (1, BLOCK):
+        if block_rows != 1 and block_rows != BLOCK:
             _refuse("Fp8Rows: block_rows is 1 or %d, got %r", BLOCK, block_rows)
         if rows < 0 or cols < 1:
             _refuse("Fp8Rows: %d x %d values", rows, cols)
-        ld, br, kb = -(-cols // 16) * 16, -(-rows // block_rows), -(-cols // BLOCK)
-        values = torch.empty(rows, ld, dtype=_E4M3, device=device)
-        scale = torch.empty(br, -(-kb // 4) * 4, dtype=_E8M0, device=device)
+        ld, sld = -(-cols // 16) * 16, -(-cols // (4 * BLOCK)) * 4
+        nbytes = rows * ld
         self = Fp8Rows.__new__(Fp8Rows)
-        self._set(values[:, :cols] if ld != cols else values, scale[:, :kb] if scale.shape[1] != kb else scale, block_rows)
+        self._store = store = torch.empty(nbytes + -(-rows // block_rows) * sld, dtype=torch.uint8, device=device)
+        self._values = self._scale = None
+        self.rows, self.cols, self.block_rows, self.device = rows, cols, block_rows, store.device
+        ptr = store.data_ptr()
+        self._c = Fp8(ptr, ptr + nbytes, rows, ld, sld, cols, block_rows, 1, 0)
         return self
 
     def dequantize(self, dtype=torch.float32):
@@ -183,51 +183,44 @@ def _padded(x, to):
     return store.view(x.dtype)[:, :x.shape[1]]
 
 
-def _empty_like(x, rows, cols, dtype):
-    if isinstance(x, T):
-        return T.empty(x.H, x.W, cols, x.device)
-    if x.dim() == 4:
-        return torch.empty((x.shape[0], cols, x.shape[2], x.shape[3]), dtype=dtype, device=x.device, memory_format=torch.channels_last)
-    return torch.empty((rows, cols), dtype=dtype, device=x.device)
-
-
 def _fp8_out(out, rows, cols, device, block_rows):
     if out is None:
         return Fp8Rows.empty(rows, cols, device, block_rows)
-    if not isinstance(out, Fp8Rows) or out.rows != rows or out.cols != cols or out.block_rows != block_rows:
+    if not isinstance(out, Fp8Rows) or out.rows != rows or out.cols != cols or out.block_rows != block_rows or not out._c.scale_e8m0:
         _refuse("row_ops: out has to be Fp8Rows.empty(%d, %d, device, block_rows=%d)", rows, cols, block_rows)
-    _same_device(device, out=out)
+    if out.device != device:
+        _refuse("row_ops: out is on %s, the input on %s", out.device, device)
     return out
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
-
-
 def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
+    dev = x.device if isinstance(x, (T, torch.Tensor)) else None
     xr = _rows(x, "x")
-    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8)
     if images is None:
-        images = x.shape[0] if not isinstance(x, T) and x.dim() == 4 else 1
+        images = 1 if isinstance(x, T) or x.dim() == 2 else x.shape[0]
     elif not isinstance(x, T) and x.dim() == 4 and images != x.shape[0]:
         _refuse("group_norm: images=%d, but x has %d", images, x.shape[0])
+    rows, cols = xr.rows, xr.cols
     code = _act_code(act)
-    wp, bp = _vector(weight, "weight", xr.cols, dev), _vector(bias, "bias", xr.cols, dev)
-    with _On(dev):
-        if fp8:
-            out = _fp8_out(out, xr.rows, xr.cols, dev, 1)
-            yr, y8 = None, C.byref(out._c)
+    wp = None if weight is None else _vector(weight, "weight", cols, dev)
+    bp = None if bias is None else _vector(bias, "bias", cols, dev)
+    if fp8:
+        out = _fp8_out(out, rows, cols, dev, 1)
+        yr, y8 = None, out._c
+    else:
+        if out is None:
+            out = T.empty(x.H, x.W, cols, dev) if isinstance(x, T) else torch.empty_like(x)
         else:
-            if out is None:
-                out = _empty_like(x, xr.rows, xr.cols, getattr(x, "dtype", None))
             _same_device(dev, out=out)
-            yr, y8 = C.byref(_rows(out, "out")), None
-        if xr.rows == 0:
-            images = 1
-        need = lib.lssvc_group_norm_workspace_bytes(xr.rows, images, xr.cols, groups, xr.dtype, 1 if fp8 else 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        check(lib.lssvc_group_norm(C.byref(xr), images, groups, wp, bp, eps, code, slope, yr, y8,
-                                   ws.data_ptr() if need else None, need, _stream(dev)))
+        yr, y8 = _rows(out, "out"), None
+    if rows == 0:
+        images = 1
+    need = lib.lssvc_group_norm_workspace_bytes(rows, images, cols, groups, xr.dtype, fp8)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(lib.lssvc_group_norm(xr, images, groups, wp, bp, eps, code, slope, yr, y8, ws.data_ptr() if need else None, need, _raw_stream(dev.index)))
     return out
 
 
@@ -248,11 +241,12 @@ def quantize_fp8(x, block_rows=1, out=None):
     power of two s >= 2^-126 with max |x| <= 448 s (1 for a block of zeros), values are e4m3(x / s) to nearest even. A value that is not
     finite becomes NaN and does not move the scale."""
     xr = _rows(x, "x")
-    if block_rows not in (1, BLOCK):
-        _refuse("quantize_fp8: block_rows is 1 or %d, got %r", BLOCK, block_rows)
-    with _On(x.device):
-        out = _fp8_out(out, xr.rows, xr.cols, x.device, block_rows)
-        check(lib.lssvc_quantize_fp8(C.byref(xr), C.byref(out._c), _stream(x.device)))
+    dev = x.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return quantize_fp8(x, block_rows, out)
+    out = _fp8_out(out, xr.rows, xr.cols, dev, block_rows)
+    check(lib.lssvc_quantize_fp8(xr, out._c, _raw_stream(dev.index)))
     return out
 
 
@@ -262,27 +256,33 @@ def matmul_fp8(a, w, bias=None, *, act=None, slope=0.01, residual=None, out=None
     (residual may be out). dtype: the output's type; by default that of out or residual, or bf16."""
     if not isinstance(a, Fp8Rows) or not isinstance(w, Fp8Rows):
         _refuse("matmul_fp8: operands are Fp8Rows (quantize_fp8, group_norm_fp8)")
-    dev = a.values.device
+    dev = a.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return matmul_fp8(a, w, bias, act=act, slope=slope, residual=residual, out=out, dtype=dtype)
     m, n = a.rows, w.rows
     code = _act_code(act)
-    bp = _vector(bias, "bias", n, dev)
-    rr = None
-    if residual is not None:
-        rr = _rows(residual, "residual")
-    with _On(dev):
-        if out is None:
-            if dtype is None:
-                dtype = torch.bfloat16 if residual is None else torch.float32 if isinstance(residual, T) else residual.dtype
-            if residual is not None:
-                out = _empty_like(residual, m, n, dtype)
-            else:
-                out = torch.empty((m, n), dtype=dtype, device=dev)
+    bp = None if bias is None else _vector(bias, "bias", n, dev)
+    rr = None if residual is None else _rows(residual, "residual")
+    if out is None:
+        if dtype is None:
+            dtype = torch.bfloat16 if rr is None else torch.float32 if isinstance(residual, T) else residual.dtype
+        dt = _DTYPE.get(dtype)
+        if dt is None:
+            _refuse("matmul_fp8: type %s (fp32, fp16 or bf16 expected)", dtype)
+        if rr is None or (not isinstance(residual, T) and residual.dim() == 2):
+            out = torch.empty((m, n), dtype=dtype, device=dev)
+            yr = Rows(out.data_ptr(), m, n, n, dt)
+        else:
+            out = T.empty(residual.H, residual.W, rr.cols, dev) if isinstance(residual, T) else torch.empty_like(residual)
+            yr = _rows(out, "out")
+    else:
         yr = _rows(out, "out")
-        if dtype is not None and _DTYPE.get(dtype) != yr.dtype:
-            _refuse("matmul_fp8: dtype %s is not the output's", dtype)
-        _same_device(dev, w=w, out=out, residual=residual)
-        need = lib.lssvc_matmul_fp8_workspace_bytes(m, n, a.cols)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        check(lib.lssvc_matmul_fp8(C.byref(a._c), C.byref(w._c), bp, code, slope, C.byref(rr) if rr is not None else None, C.byref(yr),
-                                   ws.data_ptr() if need else None, need, _stream(dev)))
+    if dtype is not None and _DTYPE.get(dtype) != yr.dtype:
+        _refuse("matmul_fp8: dtype %s is not the output's", dtype)
+    if w.device != dev or residual is not None and residual.device != dev or out.device != dev:
+        _refuse("matmul_fp8: operands on several devices")
+    need = lib.lssvc_matmul_fp8_workspace_bytes(m, n, a.cols)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(lib.lssvc_matmul_fp8(a._c, w._c, bp, code, slope, rr, yr, ws.data_ptr() if need else None, need, _raw_stream(dev.index)))
     return out
