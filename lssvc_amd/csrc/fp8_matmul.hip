@@ -12,6 +12,8 @@
 // fragment, and with the weight rows of a 64-column group dealt to the fragments as n = 16 * (r / 4) + 4 * f + r % 4 it holds 16
 // consecutive columns over four fragments: rows of y leave in 32- or 64-byte pieces. The order of k inside a block is free as long
 // as both operands share it: a lane's 32 bytes are the 16-byte chunks q and q + 4 (q = lane / 16).
+#include <cstdlib>
+#include <type_traits>
 #include "rows.h"
 
 namespace lssvc {
@@ -29,8 +31,6 @@ struct MatmulP {
     Act act;
     int tiles_m, tiles_n;
 };
-
-__device__ const i32x4 g_zero_chunk = {0, 0, 0, 0};
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -58,6 +58,11 @@ template <> struct Frag<true> {
     __device__ __forceinline__ void set(const i32x4 &lo, const i32x4 &hi) { half(lo, v[0], v[1]), half(hi, v[2], v[3]); }
 };
 
+// a fragment as it is read: chunks q and q + 4 of a row's block
+struct Raw {
+    i32x4 lo, hi;
+};
+
 // A block's scale: as the instruction takes it (an exponent byte in bits 7:0) or as a factor
 template <bool E8M0, bool WIDE> __device__ __forceinline__ auto scale_of(uint32_t bits) {
     if constexpr (!E8M0) return __uint_as_float(bits);
@@ -68,11 +73,11 @@ template <bool E8M0, bool WIDE> __device__ __forceinline__ auto scale_of(uint32_
     else return (int)bits;
 }
 
-// acc += sw * sa * (block of W) (block of A)^T
-template <bool E8M0, bool WIDE, typename S>
+// acc += sw * sa * (block of W) (block of A)^T; WB: the byte of sw that the scaled instruction takes
+template <bool E8M0, bool WIDE, int WB = 0, typename S>
 __device__ __forceinline__ void mma(const Frag<WIDE> &w, const Frag<WIDE> &a, f32x4 &acc, S sw, S sa) {
     if constexpr (E8M0 && !WIDE) {
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, acc, 0, 0, 0, sw, 0, sa);
+        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, acc, 0, 0, WB, sw, 0, sa);
     } else {
         f32x4 part = {0.f, 0.f, 0.f, 0.f};
         if constexpr (WIDE) {
@@ -120,90 +125,122 @@ template <bool E8M0> __device__ __forceinline__ uint32_t load_scale(const void *
     else return ((const uint32_t *)s)[at];
 }
 
-// ---- few rows: bound by the weight's bytes ------------------------------------------------------------------------------------------
-// A workgroup owns 16 columns of y (16 weight rows); its waves deal K's blocks among themselves, read both operands straight into
-// registers and add up through the LDS in a fixed order.
-template <int MF, bool E8M0, typename T, int NW>
-__global__ __launch_bounds__(NW * 64) void matmul_few_rows_kernel(MatmulP p) {
-    constexpr int U = 4;                          // blocks of K in flight per wave
+// ---- small products: bound by the weight's bytes, or by latency ------------------------------------------------------------------------
+// A workgroup owns MF * 16 rows and NF * 16 columns of y; its waves deal K's blocks among themselves, read both operands straight into
+// registers (nothing is read twice within the workgroup, no barrier until the end, little code) and add up through the LDS in a fixed order.
+template <int MF, int NF, bool E8M0, typename T, int NW>
+__global__ __launch_bounds__(NW * 64) void matmul_direct_kernel(MatmulP p) {
+    constexpr int U = MF + NF <= 3 ? 4 : MF + NF <= 5 ? 2 : 1;     // blocks of K in flight per wave
+    constexpr int C = 4 * NF;                                      // consecutive columns of y per lane
     constexpr bool WIDE = sizeof(T) == 4;
-    __shared__ f32x4 red[NW][MF][64];
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
+    f32x4 *red = (f32x4 *)lds;                                     // [wave][column fragment][row fragment][lane]
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * 16;
-    const int wr = min(n0 + i16, p.N - 1);
-    const uint8_t *wp = p.w + (int64_t)wr * p.ldw + q * 16;
-    const uint8_t *ap[MF];
+    const int tm = blockIdx.x / (unsigned)p.tiles_n, tn = blockIdx.x - tm * p.tiles_n;
+    const int m0 = tm * (16 * MF), n0 = tn * (16 * NF);
+    const uint8_t *wp[NF], *ap[MF];
     int64_t sar[MF];
 #pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        const int n = n0 + (NF == 1 ? i16 : (i16 >> 2) * C + f * 4 + (i16 & 3));
+        wp[f] = p.w + (int64_t)min(n, p.N - 1) * p.ldw + q * 16;
+    }
+#pragma unroll
     for (int j = 0; j < MF; ++j) {
-        const int m = min(j * 16 + i16, p.M - 1);
-        ap[j] = p.a + (int64_t)m * p.lda + q * 16;
-        sar[j] = (int64_t)m * p.ldsa;
+        const int64_t m = min(m0 + j * 16 + i16, p.M - 1);
+        ap[j] = p.a + m * p.lda + q * 16;
+        sar[j] = m * p.ldsa;
     }
     const int64_t swr = (int64_t)(n0 / kFp8Block) * p.ldsw;
-    f32x4 acc[MF] = {};
+    f32x4 acc[NF][MF] = {};
     for (int b0 = wave; b0 < p.nkb; b0 += NW * U) {
-        i32x4 wv[U][2], av[U][MF][2];
+        Raw wv[U][NF], av[U][MF];
         uint32_t ws[U], as[U][MF];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int kb = b0 + u * NW;
-            const bool on = kb < p.nkb;
-            const int k = kb * kFp8Block;
-            const bool lo = on && k + q * 16 < p.K16, hi = on && k + 64 + q * 16 < p.K16;
+            const int kb = b0 + u * NW, k = kb * kFp8Block;
+            const bool on = kb < p.nkb, lo = on && k + q * 16 < p.K16, hi = on && k + 64 + q * 16 < p.K16;
             const i32x4 z = {0, 0, 0, 0};
-            wv[u][0] = lo ? *(const i32x4 *)(wp + k) : z, wv[u][1] = hi ? *(const i32x4 *)(wp + k + 64) : z;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) wv[u][f] = Raw{lo ? *(const i32x4 *)(wp[f] + k) : z, hi ? *(const i32x4 *)(wp[f] + k + 64) : z};
             ws[u] = on ? load_scale<E8M0>(p.sw, swr + kb) : 0;
 #pragma unroll
             for (int j = 0; j < MF; ++j) {
-                av[u][j][0] = lo ? *(const i32x4 *)(ap[j] + k) : z, av[u][j][1] = hi ? *(const i32x4 *)(ap[j] + k + 64) : z;
+                av[u][j] = Raw{lo ? *(const i32x4 *)(ap[j] + k) : z, hi ? *(const i32x4 *)(ap[j] + k + 64) : z};
                 as[u][j] = on ? load_scale<E8M0>(p.sa, sar[j] + kb) : 0;
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            Frag<WIDE> wf, af;
-            wf.set(wv[u][0], wv[u][1]);
+            Frag<WIDE> wf[NF], af;
+#pragma unroll
+            for (int f = 0; f < NF; ++f) wf[f].set(wv[u][f].lo, wv[u][f].hi);
 #pragma unroll
             for (int j = 0; j < MF; ++j) {
-                af.set(av[u][j][0], av[u][j][1]);
-                mma<E8M0, WIDE>(wf, af, acc[j], scale_of<E8M0, WIDE>(ws[u]), scale_of<E8M0, WIDE>(as[u][j]));
+                af.set(av[u][j].lo, av[u][j].hi);
+#pragma unroll
+                for (int f = 0; f < NF; ++f) mma<E8M0, WIDE>(wf[f], af, acc[f][j], scale_of<E8M0, WIDE>(ws[u]), scale_of<E8M0, WIDE>(as[u][j]));
             }
         }
     }
 #pragma unroll
-    for (int j = 0; j < MF; ++j) red[wave][j][lane] = acc[j];
+    for (int f = 0; f < NF; ++f)
+#pragma unroll
+        for (int j = 0; j < MF; ++j) red[((wave * NF + f) * MF + j) * 64 + lane] = acc[f][j];
     __syncthreads();
+    const int waves = min(NW, p.nkb);                              // (the others had no block)
     for (int e = threadIdx.x; e < MF * 64; e += NW * 64) {
-        const int j = e >> 6, l = e & 63;
-        f32x4 s = red[0][j][l];
-#pragma unroll
-        for (int w = 1; w < NW; ++w) s += red[w][j][l];
-        const int m = j * 16 + (l & 15), n = n0 + (l >> 4) * 4;
+        const int m = m0 + (e >> 6) * 16 + (e & 15), n = n0 + ((e >> 4) & 3) * C;
         if (m >= p.M || n >= p.N) continue;
-        float b[4], v[4];
-        load_bias(p, n, b);
+        float v[C];
+        load_bias(p, n, v);
+        f32x4 s[NF] = {};
+        for (int w = 0; w < waves; ++w)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = s[r] + b[r];
-        store_cols<T, 4>(p, m, n, v);
+            for (int f = 0; f < NF; ++f) s[f] += red[(w * NF + f) * MF * 64 + e];
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[c] += s[c >> 2][c & 3];
+        store_cols<T, C>(p, m, n, v);
     }
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------------------
 // BM x BN of y per workgroup, WM x WN per wave. K's blocks pass through two LDS stages of (BM + BN) x 128 bytes, filled by LDS-DMA
-// (16 bytes a lane, no registers) one block ahead. A row's eight 16-byte chunks are stored permuted, chunk c at c ^ key(row), so that the 16
-// rows of a fragment read cover all 64 banks; the permutation is applied to the DMA's SOURCE address, its destination is linear.
+// (16 bytes a lane, no registers). A row's eight 16-byte chunks are stored permuted, chunk c at c ^ key(row), so that the 16 rows of a
+// fragment read cover all 64 banks; the permutation is applied to the DMA's SOURCE address, its destination is linear.
+//
+// The matrix units are the bound, so they must not see the LDS: a wave multiplies the fragments of A one after the other against its FN
+// fragments of W and reads PD fragments ahead, over the end of the block too. The one barrier of a block stands PD fragments before its
+// end: there every wave has all of this block in registers and its part of the next one has landed; behind it the stage just read
+// is filled with the block after the next, a quarter of the instructions with each of the next four fragments. (All at once they fill the
+// address unit's queue, and the waves stand in front of it with the matrix units idle: 0.5 us of a block's 1.8 at 256 x 256.)
 __device__ __forceinline__ int key_a(int row) { return (row >> 1) & 7; }                                     // fragment rows: consecutive
 __device__ __forceinline__ int key_w(int row) { return ((row >> 1) & 1) | (((row >> 4) & 3) << 1); }         // fragment rows: 16 (r / 4) + 4 f + r % 4
+
+struct RawA {
+    i32x4 lo, hi;
+    uint32_t scale;
+};
+// a raw buffer of the bytes [p, p + range)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const uint8_t *p, int range) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, range, 0x00027000);
+}
+// a value that all lanes share, in scalar registers
+__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
+    const uint64_t v = (uint64_t)p;
+    return (const uint8_t *)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
 
 template <int BM, int BN, int WM, int WN, bool E8M0, typename T>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel(MatmulP p) {
     constexpr int NWAVE = (BM / WM) * (BN / WN), FM = WM / 16, FN = WN / 16, STAGE = (BM + BN) * kFp8Block;
-    constexpr int PER = (BM + BN) / 8 / NWAVE;
+    constexpr int PA = BM / 8 / NWAVE, PW = BN / 8 / NWAVE;    // DMA instructions of a wave per block
+    constexpr int SLOTS = 2, PD = 1, LAST = FM - PD;
+    constexpr int DPG = (PA + PW) / 4;                         // DMA instructions per fragment of A
     constexpr bool WIDE = sizeof(T) == 4;
-    static_assert(WN % 64 == 0 && (BM + BN) % (8 * NWAVE) == 0 && BM % 8 == 0 && 128 % WN == 0, "tile");
+    static_assert(WN % 64 == 0 && BM % (8 * NWAVE) == 0 && BN % (8 * NWAVE) == 0 && 128 % WN == 0 && FM % SLOTS == 0 && FM >= 4 && (PA + PW) % 4 == 0, "tile");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, q = lane >> 4;
     // workgroups go to the eight XCDs in turn: give each XCD a run of tiles, walked in bands of 8 tile rows, so that its L2 sees the
     // same operands again
     const int total = p.tiles_m * p.tiles_n;
@@ -213,122 +250,196 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
         id = xcd * per + min(xcd, more) + at;
     }
     const int band = id / (8 * p.tiles_n), in_band = id - band * 8 * p.tiles_n, rows = min(8, p.tiles_m - band * 8);
-    const int tm = band * 8 + in_band % rows, tn = in_band / rows;
+    const int tm = __builtin_amdgcn_readfirstlane(band * 8 + in_band % rows), tn = __builtin_amdgcn_readfirstlane(in_band / rows);
     const int m0 = tm * BM, n0 = tn * BN;
 
-    const uint8_t *src[PER];
-    int chunk[PER];
+    // Both operands are read through buffer descriptors that start at the tile's rows: a lane's offset within the tile in a register (the host
+    // keeps 256 pitches below 2^31), k in the instruction's scalar offset. Rows behind the last one are the last one (their results are not
+    // stored); chunks behind K16 get an offset beyond the range and arrive as zeros; a block behind the last one is the last one.
+    constexpr int STEP = 8 * NWAVE;                            // rows between two DMA instructions of a wave
+    const uint8_t *abase = uniform(p.a + (int64_t)m0 * p.lda), *wbase = uniform(p.w + (int64_t)n0 * p.ldw);
+    const int drow = wave * 8 + (lane >> 3);
+    const int achunk = ((lane & 7) ^ key_a(drow)) * 16;        // (the key of a row of A repeats after 16 rows, that of W after 64)
+    uint32_t aoff[PA], woff[PW];
+    int wchunk[PW];
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int row = (wave + i * NWAVE) * 8 + (lane >> 3);          // rows 0 ... BM - 1: A; then W
-        if (row < BM) {
-            chunk[i] = (lane & 7) ^ key_a(row);
-            src[i] = p.a + (int64_t)min(m0 + row, p.M - 1) * p.lda + chunk[i] * 16;
-        } else {
-            chunk[i] = (lane & 7) ^ key_w(row - BM);
-            src[i] = p.w + (int64_t)min(n0 + row - BM, p.N - 1) * p.ldw + chunk[i] * 16;
-        }
+    for (int i = 0; i < PA; ++i) aoff[i] = (uint32_t)min(drow + i * STEP, p.M - 1 - m0) * (uint32_t)p.lda + achunk;
+#pragma unroll
+    for (int i = 0; i < PW; ++i) {
+        wchunk[i] = ((lane & 7) ^ key_w(drow + i * STEP)) * 16;
+        woff[i] = (uint32_t)min(drow + i * STEP, p.N - 1 - n0) * (uint32_t)p.ldw + wchunk[i];
     }
-    auto fill = [&](int kb, int stage) {
-        const int k = kb * kFp8Block;
-        const bool ragged = k + kFp8Block > p.K16;
+    auto dma = [&](const uint8_t *base, uint32_t off, int k, int at) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(descriptor(base, 0x7fffffff), (__attribute__((address_space(3))) void *)(lds + at), 16, off, k, 0, 0);
+    };
+    auto fill = [&](int kb, int from, int to) {                // DMA instructions from ... to - 1 of a block's
+        const int k = min(kb, p.nkb - 1) * kFp8Block, at = (kb & 1) * STAGE + wave * 1024;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const uint8_t *s = src[i] + k;
-            if (ragged && k + chunk[i] * 16 >= p.K16) s = (const uint8_t *)&g_zero_chunk;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)s,
-                                             (__attribute__((address_space(3))) void *)(lds + stage * STAGE + (wave + i * NWAVE) * 1024), 16, 0, 0);
+        for (int i = 0; i < PA + PW; ++i) {
+            if (i < from || i >= to) continue;
+            if (i < PA) dma(abase, k + achunk < p.K16 ? aoff[i] : 0x80000000u, k, at + i * STEP * kFp8Block);
+            else dma(wbase, k + wchunk[i - PA] < p.K16 ? woff[i - PA] : 0x80000000u, k, at + (BM + (i - PA) * STEP) * kFp8Block);
         }
     };
 
+    // A's scales go through the LDS as well, for four blocks of K at a time (a dword of e8m0 bytes or four fp32 values per row, two such groups):
+    // read straight from memory every wave would gather them for itself, 16 cache lines an instruction, and the address unit would be the
+    // bound. A wave's DMA covers 64 rows; where there are more waves than that some write the same values twice.
     const int wm = (wave % (BM / WM)) * WM, wn = (wave / (BM / WM)) * WN;
-    int64_t sar[FM];
-#pragma unroll
-    for (int j = 0; j < FM; ++j) sar[j] = (int64_t)min(m0 + wm + j * 16 + i16, p.M - 1) * p.ldsa;
-    const int64_t swr = (int64_t)(min(n0 + wn, p.N - 1) / kFp8Block) * p.ldsw;
-    // e8m0: four blocks' scale bytes per dword; fp32: one block's. The next ones are on their way while these are used.
-    uint32_t sa[FM], san[FM], sw = 0, swn;
-    auto fetch = [&](int kb) {
-        if constexpr (E8M0) {
-            const int at = min(kb, (p.nkb - 1) & ~3);
-#pragma unroll
-            for (int j = 0; j < FM; ++j) san[j] = *(const uint32_t *)((const uint8_t *)p.sa + sar[j] + at);
-            swn = *(const uint32_t *)((const uint8_t *)p.sw + swr + at);
-        } else {
-            const int at = min(kb, p.nkb - 1);
-#pragma unroll
-            for (int j = 0; j < FM; ++j) san[j] = load_scale<false>(p.sa, sar[j] + at);
-            swn = load_scale<false>(p.sw, swr + at);
-        }
+    constexpr int SB = E8M0 ? 1 : 4, SROW = 4 * SB;
+    const int srow = (wave * 64) % BM;
+    // (a group behind the last one is the last one; behind the row's last scale the buffer may end, so the range does: zeros)
+    const uint8_t *sabase = uniform((const uint8_t *)p.sa + (int64_t)m0 * p.ldsa * SB);
+    const int64_t sleft = ((int64_t)(p.M - 1 - m0) * p.ldsa + (E8M0 ? (p.nkb + 3) & ~3 : p.nkb)) * SB;
+    const int srange = __builtin_amdgcn_readfirstlane((int)min(sleft, (int64_t)0x7fffffff));
+    const uint32_t saoff = (uint32_t)min(srow + lane, p.M - 1 - m0) * (uint32_t)p.ldsa * SB;
+    auto fill_scales = [&](int g) {
+        const int gk = min(g, (p.nkb - 1) >> 2) * SROW;
+        const auto to = (__attribute__((address_space(3))) void *)(lds + 2 * STAGE + ((g & 1) * BM + srow) * SROW);
+        if constexpr (E8M0) __builtin_amdgcn_raw_ptr_buffer_load_lds(descriptor(sabase, srange), to, 4, saoff + gk, 0, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(descriptor(sabase, srange), to, 16, saoff + gk, 0, 0, 0);
     };
-    fill(0, 0);
-    fetch(0);
+    // W's scales: one per block and wave, in registers, four blocks at a time
+    const uint8_t *swp = (const uint8_t *)p.sw + (int64_t)(min(n0 + wn, p.N - 1) / kFp8Block) * p.ldsw * SB;
+    constexpr int NSW = E8M0 ? 1 : 4;
+    uint32_t sw[NSW], swn[NSW];
+    auto fetch_w = [&](int g, uint32_t (&to)[NSW]) {
+        if constexpr (E8M0) to[0] = *(const uint32_t *)(swp + min(g * 4, (p.nkb - 1) & ~3));
+        else
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to[i] = *(const uint32_t *)(swp + 4 * min(g * 4 + i, p.nkb - 1));
+    };
 
+    // fragment addresses within a stage: consecutive fragments of A are 16 rows apart and share their key; those of W differ in row bits 3:2,
+    // which the key does not see
+    const int arow = wm + i16, wrow = wn + (i16 >> 2) * 16 + (i16 & 3);
+    const int a_lo = arow * kFp8Block + ((q ^ key_a(arow)) * 16), a_hi = arow * kFp8Block + (((q + 4) ^ key_a(arow)) * 16);
+    const int w_lo = (BM + wrow) * kFp8Block + ((q ^ key_w(wrow)) * 16), w_hi = (BM + wrow) * kFp8Block + (((q + 4) ^ key_w(wrow)) * 16);
+    const int sc0 = 2 * STAGE + arow * SROW;
+    auto read_a = [&](int kb, int j) {
+        const uint8_t *st = lds + (kb & 1) * STAGE + j * (16 * kFp8Block), *sc = lds + sc0 + ((kb >> 2) & 1) * (BM * SROW) + (kb & 3) * SB + j * (16 * SROW);
+        RawA r{*(const i32x4 *)(st + a_lo), *(const i32x4 *)(st + a_hi), 0};
+        if constexpr (E8M0) r.scale = *sc;
+        else r.scale = *(const uint32_t *)sc;
+        return r;
+    };
+    auto read_w = [&](int kb, int f) {
+        const uint8_t *st = lds + (kb & 1) * STAGE + ((f >> 2) * 64 + (f & 3) * 4) * kFp8Block;
+        return Raw{*(const i32x4 *)(st + w_lo), *(const i32x4 *)(st + w_hi)};
+    };
+
+    fill(0, 0, PA + PW);
+    fill_scales(0);
+    fetch_w(0, sw);
     f32x4 acc[FN][FM] = {};
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int kb = 0; kb < p.nkb; ++kb) {
-        const uint8_t *st = lds + (kb & 1) * STAGE;
-        if (kb + 1 < p.nkb) fill(kb + 1, (kb + 1) & 1);
-        if (!E8M0 || (kb & 3) == 0) {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    fill(1, 0, DPG);
+    Raw wraw[FN];
+    RawA araw[SLOTS];
 #pragma unroll
-            for (int j = 0; j < FM; ++j) sa[j] = san[j];
-            sw = swn;
-            fetch(kb + (E8M0 ? 4 : 1));
-        }
-        Frag<WIDE> af[FM];
+    for (int f = 0; f < FN; ++f) wraw[f] = read_w(0, f);
+#pragma unroll
+    for (int j = 0; j < PD; ++j) araw[j] = read_a(0, j);
+    // one block of K; S = kb % 4. No branches inside: the compiler would gather the products behind them. (A block behind the last one is filled
+    // with zeros, its descriptor's range being empty, and read for nothing.)
+    auto step = [&](int kb, auto s_) {
+        constexpr int S = decltype(s_)::value;
+        Frag<WIDE> wf[FN];
+#pragma unroll
+        for (int f = 0; f < FN; ++f) wf[f].set(wraw[f].lo, wraw[f].hi);
+        if constexpr (S == 0) fetch_w((kb >> 2) + 1, swn);
+        const auto swv = scale_of<E8M0, WIDE>(E8M0 ? (WIDE ? sw[0] >> (8 * S) : sw[0]) : sw[E8M0 ? 0 : S]);
 #pragma unroll
         for (int j = 0; j < FM; ++j) {
-            const int row = wm + j * 16 + i16;
-            const uint8_t *r = st + row * kFp8Block;
-            af[j].set(*(const i32x4 *)(r + ((q ^ key_a(row)) * 16)), *(const i32x4 *)(r + (((q + 4) ^ key_a(row)) * 16)));
-        }
+            if (j == LAST) {
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");        // this block is in registers, this wave's part of the next has landed
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if constexpr (S == 1) fill_scales((kb >> 2) + 1);
+                fill(kb + 2, 0, DPG);
+            } else if (j < 3) fill(kb + 1, (j + 1) * DPG, (j + 2) * DPG);
+            if (j + PD < FM) araw[(j + PD) % SLOTS] = read_a(kb, j + PD);
+            else araw[(j + PD) % SLOTS] = read_a(kb + 1, j + PD - FM);
+            __builtin_amdgcn_sched_barrier(0);
+            Frag<WIDE> af;
+            af.set(araw[j % SLOTS].lo, araw[j % SLOTS].hi);
+            const auto sav = scale_of<E8M0, WIDE>(araw[j % SLOTS].scale);
 #pragma unroll
-        for (int f = 0; f < FN; ++f) {
-            const int row = wn + (f >> 2) * 64 + (i16 >> 2) * 16 + (f & 3) * 4 + (i16 & 3);
-            const uint8_t *r = st + (BM + row) * kFp8Block;
-            Frag<WIDE> wf;
-            wf.set(*(const i32x4 *)(r + ((q ^ key_w(row)) * 16)), *(const i32x4 *)(r + (((q + 4) ^ key_w(row)) * 16)));
-#pragma unroll
-            for (int j = 0; j < FM; ++j) mma<E8M0, WIDE>(wf, af[j], acc[f][j], scale_of<E8M0, WIDE>(sw), scale_of<E8M0, WIDE>(sa[j]));
+            for (int f = 0; f < FN; ++f) {
+                mma<E8M0, WIDE, S>(wf[f], af, acc[f][j], swv, sav);
+                if (!E8M0 || WIDE) asm volatile("" : "+v"(acc[f][j]));             // (the sum is made here: kept back, the parts would fill the registers)
+                if (j == FM - 1) {                             // this was the fragment's last use: the next block's takes its registers
+                    __builtin_amdgcn_sched_barrier(0);
+                    wraw[f] = read_w(kb + 1, f);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (E8M0) {
+        if constexpr (S == 3)
 #pragma unroll
-            for (int j = 0; j < FM; ++j) sa[j] >>= 8;
-            sw >>= 8;
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");               // this wave's part of the next block has landed
-        __syncthreads();
+            for (int i = 0; i < NSW; ++i) sw[i] = swn[i];
+    };
+    for (int kb = 0;;) {
+        step(kb, std::integral_constant<int, 0>{});
+        if (++kb == p.nkb) break;
+        step(kb, std::integral_constant<int, 1>{});
+        if (++kb == p.nkb) break;
+        step(kb, std::integral_constant<int, 2>{});
+        if (++kb == p.nkb) break;
+        step(kb, std::integral_constant<int, 3>{});
+        if (++kb == p.nkb) break;
     }
 
+    // Out through the LDS, 64 x 64 of a wave's tile at a time in a part of its own: whole 128- or 256-byte pieces of rows, and a short loop
+    // instead of a long unrolled one (a tile's registers cannot be indexed; 16 KB of code cost more to fetch than the tile takes to store).
+    // A row's 16-byte chunk c lies at c ^ (row % 16): both directions cover the banks.
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");                    // (fills behind the last block)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    static_assert(FM % 4 == 0 && FN == 4 && NWAVE * 16384 <= 2 * STAGE, "epilogue");
+    f32x4 *part = (f32x4 *)(lds + wave * 16384);
+    const int c8 = lane & 7, n = n0 + wn + c8 * 8;
+    float bias[8];
 #pragma unroll
-    for (int g = 0; g < FN / 4; ++g) {
-        const int n = n0 + wn + g * 64 + q * 16;
-        if (n >= p.N) continue;
-        float b[16];
-        load_bias(p, n, b);
+    for (int i = 0; i < 8; ++i) bias[i] = p.bias ? p.bias[min(n + i, p.N - 1)] : 0.f;
 #pragma unroll
-        for (int j = 0; j < FM; ++j) {
-            const int m = m0 + wm + j * 16 + i16;
-            if (m >= p.M) continue;
-            float v[16];
+    for (int h = 0; h < FM / 4; ++h) {
 #pragma unroll
-            for (int c = 0; c < 16; ++c) v[c] = acc[g * 4 + (c >> 2)][j][c & 3] + b[c];
-            store_cols<T, 16>(p, m, n, v);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int f = 0; f < 4; ++f) part[(j * 16 + i16) * 16 + ((q * 4 + f) ^ i16)] = acc[f][h * 4 + j];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        const int mh = m0 + wm + h * 64;
+#pragma unroll 1
+        for (int r = lane >> 3; r < 64; r += 8) {
+            const f32x4 x = part[r * 16 + ((c8 * 2) ^ (r & 15))], y = part[r * 16 + ((c8 * 2 + 1) ^ (r & 15))];
+            float v[8] = {x[0] + bias[0], x[1] + bias[1], x[2] + bias[2], x[3] + bias[3], y[0] + bias[4], y[1] + bias[5], y[2] + bias[6], y[3] + bias[7]};
+            if (mh + r < p.M && n < p.N) store_cols<T, 8>(p, mh + r, n, v);
         }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
-template <int MF, bool E8M0, typename T> static int launch_few(const MatmulP &p, hipStream_t s) {
-    const unsigned grid = (unsigned)((p.N + 15) / 16);
-    if (p.nkb <= 8) matmul_few_rows_kernel<MF, E8M0, T, 4><<<grid, 256, 0, s>>>(p);
-    else matmul_few_rows_kernel<MF, E8M0, T, 8><<<grid, 512, 0, s>>>(p);
+template <int MF, int NF, bool E8M0, typename T, int NW> static int launch_direct(const MatmulP &p, int64_t total, hipStream_t s) {
+    static LdsGrant grant;
+    constexpr size_t bytes = (size_t)NW * MF * NF * 1024;
+    if (int rc = grant.ensure((const void *)matmul_direct_kernel<MF, NF, E8M0, T, NW>, bytes, 64 * 1024)) return rc;
+    matmul_direct_kernel<MF, NF, E8M0, T, NW><<<(unsigned)total, NW * 64, bytes, s>>>(p);
     return launch_status("matmul_fp8");
+}
+template <int MF, int NF, bool E8M0, typename T> static int launch_direct(MatmulP p, hipStream_t s) {
+    p.tiles_m = (p.M + 16 * MF - 1) / (16 * MF);
+    p.tiles_n = (p.N + 16 * NF - 1) / (16 * NF);
+    const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
+    LSSVC_CHECK(total < (1LL << 31), "matmul_fp8: %lld tiles do not fit one launch", (long long)total);
+    return p.nkb <= 8 ? launch_direct<MF, NF, E8M0, T, 4>(p, total, s) : launch_direct<MF, NF, E8M0, T, 8>(p, total, s);
 }
 
 template <int BM, int BN, int WM, int WN, bool E8M0, typename T> static int launch_tile(MatmulP p, hipStream_t s) {
     static LdsGrant grant;
-    constexpr size_t bytes = 2 * (BM + BN) * kFp8Block;
+    constexpr size_t bytes = 2 * (BM + BN) * kFp8Block + 2 * BM * (E8M0 ? 4 : 16);
     if (int rc = grant.ensure((const void *)matmul_tile_kernel<BM, BN, WM, WN, E8M0, T>, bytes, 64 * 1024)) return rc;
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
@@ -339,13 +450,23 @@ template <int BM, int BN, int WM, int WN, bool E8M0, typename T> static int laun
 }
 
 template <bool E8M0, typename T> static int launch_matmul(const MatmulP &p, hipStream_t s) {
-    if (p.M <= 16) return launch_few<1, E8M0, T>(p, s);
-    if (p.M <= 32) return launch_few<2, E8M0, T>(p, s);
+    const int force = getenv("FP8_FORCE") ? atoi(getenv("FP8_FORCE")) : 0;
+    if (force) switch (force) {
+        case 11: return launch_direct<1, 1, E8M0, T>(p, s);
+        case 21: return launch_direct<2, 1, E8M0, T>(p, s);
+        case 41: return launch_direct<4, 1, E8M0, T>(p, s);
+        case 24: return launch_direct<2, 4, E8M0, T>(p, s);
+        case 44: return launch_direct<4, 4, E8M0, T>(p, s);
+        case 128: return launch_tile<128, 128, 64, 64, E8M0, T>(p, s);
+        case 256: if constexpr (sizeof(T) == 2) return launch_tile<256, 256, 128, 64, E8M0, T>(p, s); else return launch_tile<128, 128, 64, 64, E8M0, T>(p, s);
+    }
+    if (p.M <= 16) return launch_direct<1, 1, E8M0, T>(p, s);
+    if (p.M <= 32) return launch_direct<2, 1, E8M0, T>(p, s);
     auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
     if constexpr (sizeof(T) == 2)
         if (tiles(256, 256) >= 200) return launch_tile<256, 256, 128, 64, E8M0, T>(p, s);
     if (tiles(128, 128) >= 200) return launch_tile<128, 128, 64, 64, E8M0, T>(p, s);
-    return launch_tile<64, 64, 16, 64, E8M0, T>(p, s);
+    return launch_direct<4, 4, E8M0, T>(p, s);
 }
 template <bool E8M0> static int launch_typed(const MatmulP &p, hipStream_t s) {
     if (p.dtype == LSSVC_F32) return launch_matmul<E8M0, float>(p, s);
@@ -360,7 +481,7 @@ static int operand_check(const lssvc_fp8 *x, const char *who, int block_rows) {
     LSSVC_CHECK(aligned(x->values, 16) && x->ld % 16 == 0 && x->ld >= ((int64_t)x->cols + 15) / 16 * 16, "matmul_fp8: operand %s needs a 16-byte aligned base and a pitch that is a multiple of 16", who);
     const int64_t kb = ((int64_t)x->cols + kFp8Block - 1) / kFp8Block;
     LSSVC_CHECK(x->scale_ld >= kb && aligned(x->scale, 4) && (!x->scale_e8m0 || x->scale_ld % 4 == 0), "matmul_fp8: operand %s: bad scale layout", who);
-    LSSVC_CHECK(x->rows < (1LL << 31) - 512 && x->cols <= (1 << 30) && x->ld < (1LL << 32), "matmul_fp8: operand %s is too large", who);
+    LSSVC_CHECK(x->rows < (1LL << 31) - 512 && x->ld < (1LL << 22) && x->scale_ld < (1LL << 21), "matmul_fp8: operand %s is too large", who);
     return 0;
 }
 
@@ -397,6 +518,6 @@ extern "C" int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const fl
     p.res = residual ? residual->ptr : nullptr, p.ldres = residual ? residual->ld : 0;
     p.y = y->ptr, p.ldy = y->ld;
     p.M = (int)a->rows, p.N = (int)w->rows, p.K16 = (a->cols + 15) / 16 * 16, p.nkb = (a->cols + kFp8Block - 1) / kFp8Block;
-    p.dtype = y->dtype, p.act = make_act(act, slope);
+    p.dtype = y->dtype, p.act = Act{act, slope};
     return a->scale_e8m0 ? launch_typed<true>(p, (hipStream_t)stream) : launch_typed<false>(p, (hipStream_t)stream);
 }

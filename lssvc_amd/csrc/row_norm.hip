@@ -633,7 +633,7 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     p.w = weight, p.b = bias;
     p.C = x->cols, p.G = groups, p.cg = x->cols / groups;
     p.S = q.S, p.P = q.P, p.piece = q.piece, p.chunk = q.chunk, p.slice = q.slice, p.nslices = q.nslices;
-    p.act = make_act(act, slope), p.eps = eps;
+    p.act = Act{act, slope}, p.eps = eps;
     p.in_place = y && y->ptr == x->ptr;
     p.stat = (float2 *)workspace;
     p.part = p.stat + (int64_t)images * x->cols;

@@ -53,25 +53,23 @@ template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(con
 }
 template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) { __builtin_memcpy(p, &r, sizeof(r)); }
 
-// Activations, for N values at a time so that the choice is made once. None, relu and lrelu are one form, v < 0 ? max(v, floor) * slope : v, with
-// slope 1, 0 or the caller's (floor keeps relu's -inf * 0 from being NaN). silu: exp and reciprocal at the hardware's 1 ulp, 2^-22 relative
-// beside the 2^-24 .. 2^-8 of the stored result. NaN passes through.
+// Activations, for N values at a time so that the choice is made once. silu: exp and reciprocal at the hardware's 1 ulp, 2^-22 relative
+// beside the 2^-24 .. 2^-8 of the stored result. NaN passes through all of them.
 struct Act {
-    float slope, floor;
-    int silu;
+    int kind;
+    float slope;
 };
-inline Act make_act(int act, float slope) {
-    const float inf = __builtin_inff();
-    if (act == LSSVC_ACT_SILU) return Act{0.f, 0.f, 1};
-    return act == LSSVC_ACT_NONE ? Act{1.f, -inf, 0} : act == LSSVC_ACT_RELU ? Act{0.f, -3.402823466e38f, 0} : Act{slope, -inf, 0};
-}
 template <int N> __device__ __forceinline__ void apply_act(float (&v)[N], const Act &a) {
-    if (a.silu) {
+    if (a.kind == LSSVC_ACT_NONE) return;
+    if (a.kind == LSSVC_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = v[i] * __builtin_amdgcn_rcpf(1.f + __expf(-v[i]));
+    } else if (a.kind == LSSVC_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? fmaxf(v[i], a.floor) * a.slope : v[i];
+        for (int i = 0; i < N; ++i) v[i] = v[i] < 0.f ? v[i] * a.slope : v[i];
     }
 }
 
