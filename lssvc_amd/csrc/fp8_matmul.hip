@@ -90,30 +90,27 @@ __device__ __forceinline__ void mma(const Frag<WIDE> &w, const Frag<WIDE> &a, f3
     }
 }
 
-// act(v) + residual for CNT consecutive columns of one row, rounded once
-template <typename T, int CNT>
-__device__ __forceinline__ void store_cols(const MatmulP &p, int64_t m, int n, float (&v)[CNT]) {
-    T *dst = (T *)p.y + m * p.ldy + n;
-    const T *res = p.res ? (const T *)p.res + m * p.ldres + n : nullptr;
-    const bool full = n + CNT <= p.N;
-    apply_act(v, p.act);
+// act(v) + residual for CNT consecutive columns of one row, rounded once. FULL: all of them are inside; otherwise the first `left`.
+template <bool FULL, typename T, int CNT>
+__device__ __forceinline__ void store_cols(const Act &act, T *dst, const T *res, int left, float (&v)[CNT]) {
+    apply_act(v, act);
     if (res) {
         Pack<T, CNT> r;
-        if (full) r = load_pack<T, CNT>(res);
+        if (FULL) r = load_pack<T, CNT>(res);
         else
 #pragma unroll
-            for (int i = 0; i < CNT; ++i) r.v[i] = n + i < p.N ? res[i] : from_f32<T>(0.f);
+            for (int i = 0; i < CNT; ++i) r.v[i] = i < left ? res[i] : from_f32<T>(0.f);
 #pragma unroll
         for (int i = 0; i < CNT; ++i) v[i] += to_f32(r.v[i]);
     }
     Pack<T, CNT> o;
 #pragma unroll
     for (int i = 0; i < CNT; ++i) o.v[i] = from_f32<T>(v[i]);
-    if (full) store_pack(dst, o);
+    if (FULL) store_pack(dst, o);
     else
 #pragma unroll
         for (int i = 0; i < CNT; ++i)
-            if (n + i < p.N) dst[i] = o.v[i];
+            if (i < left) dst[i] = o.v[i];
 }
 template <int CNT> __device__ __forceinline__ void load_bias(const MatmulP &p, int n, float (&b)[CNT]) {
 #pragma unroll
@@ -190,7 +187,7 @@ __global__ __launch_bounds__(NW * 64) void matmul_direct_kernel(MatmulP p) {
     __syncthreads();
     const int waves = min(NW, p.nkb);                              // (the others had no block)
     for (int e = threadIdx.x; e < MF * 64; e += NW * 64) {
-        const int m = m0 + (e >> 6) * 16 + (e & 15), n = n0 + ((e >> 4) & 3) * C;
+        const int64_t m = m0 + (e >> 6) * 16 + (e & 15), n = n0 + ((e >> 4) & 3) * C;
         if (m >= p.M || n >= p.N) continue;
         float v[C];
         load_bias(p, n, v);
@@ -200,7 +197,10 @@ __global__ __launch_bounds__(NW * 64) void matmul_direct_kernel(MatmulP p) {
             for (int f = 0; f < NF; ++f) s[f] += red[(w * NF + f) * MF * 64 + e];
 #pragma unroll
         for (int c = 0; c < C; ++c) v[c] += s[c >> 2][c & 3];
-        store_cols<T, C>(p, m, n, v);
+        T *dst = (T *)p.y + m * p.ldy + n;
+        const T *res = p.res ? (const T *)p.res + m * p.ldres + n : nullptr;
+        if (n0 + 16 * NF <= p.N) store_cols<true, T, C>(p.act, dst, res, C, v);        // (the workgroup agrees)
+        else store_cols<false, T, C>(p.act, dst, res, p.N - n, v);
     }
 }
 
@@ -403,7 +403,27 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
     const int c8 = lane & 7, n = n0 + wn + c8 * 8;
     float bias[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) bias[i] = p.bias ? p.bias[min(n + i, p.N - 1)] : 0.f;
+    for (int i = 0; i < 8; ++i) {
+        bias[i] = p.bias ? p.bias[min(n + i, p.N - 1)] : 0.f;
+        asm volatile("" : "+v"(bias[i]));                      // (waited for here, not in the loop: there the wait would be for its stores)
+    }
+    const int r0 = lane >> 3, x0 = (c8 * 2) ^ r0, y0 = (c8 * 2 + 1) ^ r0;          // (rows r0 + 8 k: the key alternates between r0 and r0 ^ 8)
+    auto out = [&](auto full_, int mh) {
+        constexpr bool FULL = decltype(full_)::value;
+        const int rows_left = min(64, p.M - mh);
+        T *dst = (T *)p.y + (int64_t)(mh + r0) * p.ldy + n;
+        const T *res = (const T *)p.res + (p.res ? (int64_t)(mh + r0) * p.ldres + n : 0);
+        const f32x4 *from = part + r0 * 16;
+#pragma unroll 2
+        for (int k = 0; k < 8; ++k) {
+            const f32x4 x = from[x0 ^ ((k & 1) * 8)], y = from[y0 ^ ((k & 1) * 8)];
+            float v[8] = {x[0] + bias[0], x[1] + bias[1], x[2] + bias[2], x[3] + bias[3], y[0] + bias[4], y[1] + bias[5], y[2] + bias[6], y[3] + bias[7]};
+            if (r0 + 8 * k < rows_left && (FULL || n < p.N)) store_cols<FULL, T, 8>(p.act, dst, p.res ? res : nullptr, p.N - n, v);
+            dst += 8 * p.ldy;
+            res += 8 * p.ldres;
+            from += 8 * 16;
+        }
+    };
 #pragma unroll
     for (int h = 0; h < FM / 4; ++h) {
 #pragma unroll
@@ -411,13 +431,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
 #pragma unroll
             for (int f = 0; f < 4; ++f) part[(j * 16 + i16) * 16 + ((q * 4 + f) ^ i16)] = acc[f][h * 4 + j];
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const int mh = m0 + wm + h * 64;
-#pragma unroll 1
-        for (int r = lane >> 3; r < 64; r += 8) {
-            const f32x4 x = part[r * 16 + ((c8 * 2) ^ (r & 15))], y = part[r * 16 + ((c8 * 2 + 1) ^ (r & 15))];
-            float v[8] = {x[0] + bias[0], x[1] + bias[1], x[2] + bias[2], x[3] + bias[3], y[0] + bias[4], y[1] + bias[5], y[2] + bias[6], y[3] + bias[7]};
-            if (mh + r < p.M && n < p.N) store_cols<T, 8>(p, mh + r, n, v);
-        }
+        if (n0 + BN <= p.N) out(std::true_type{}, m0 + wm + h * 64);
+        else out(std::false_type{}, m0 + wm + h * 64);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }

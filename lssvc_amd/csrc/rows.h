@@ -46,12 +46,30 @@ template <> __device__ __forceinline__ bf16_t from_f32<bf16_t>(float x) {
 // N consecutive values as they lie in memory, at the type's own alignment: global loads and stores of any width need no more on
 // gfx950, so slices and odd pitches take the wide path too.
 template <typename T, int N> struct Pack { T v[N]; };
+template <int BYTES> struct Words;                              // the widest pieces of BYTES, as a vector of 2-byte alignment
+template <> struct Words<2> { typedef uint16_t type; };
+template <> struct Words<4> { typedef uint32_t type __attribute__((aligned(2))); };
+template <> struct Words<8> { typedef uint32_t type __attribute__((ext_vector_type(2), aligned(2))); };
+template <> struct Words<16> { typedef uint32_t type __attribute__((ext_vector_type(4), aligned(2))); };
+template <int BYTES> constexpr int kPiece = BYTES > 16 ? 16 : BYTES;
 template <typename T, int N> __device__ __forceinline__ Pack<T, N> load_pack(const T *p) {
+    using W = typename Words<kPiece<sizeof(Pack<T, N>)>>::type;
+    constexpr int Q = sizeof(Pack<T, N>) / sizeof(W);
+    W w[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i) w[i] = ((const W *)p)[i];
     Pack<T, N> r;
-    __builtin_memcpy(&r, p, sizeof(r));
+    __builtin_memcpy(&r, w, sizeof(r));
     return r;
 }
-template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) { __builtin_memcpy(p, &r, sizeof(r)); }
+template <typename T, int N> __device__ __forceinline__ void store_pack(T *p, const Pack<T, N> &r) {
+    using W = typename Words<kPiece<sizeof(Pack<T, N>)>>::type;
+    constexpr int Q = sizeof(Pack<T, N>) / sizeof(W);
+    W w[Q];
+    __builtin_memcpy(w, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < Q; ++i) ((W *)p)[i] = w[i];
+}
 
 // Activations, for N values at a time so that the choice is made once. silu: exp and reciprocal at the hardware's 1 ulp, 2^-22 relative
 // beside the 2^-24 .. 2^-8 of the stored result. NaN passes through all of them.
