@@ -73,21 +73,24 @@ template <bool E8M0, bool WIDE> __device__ __forceinline__ auto scale_of(uint32_
     else return (int)bits;
 }
 
+// (block of W) (block of A)^T without the scales
+template <bool WIDE> __device__ __forceinline__ f32x4 product(const Frag<WIDE> &w, const Frag<WIDE> &a) {
+    f32x4 part = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], a.v[i], part, 0, 0, 0);
+    } else part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, part, 0, 0, 0, 0, 0, 0);      // (unscaled)
+    return part;
+}
+__device__ __forceinline__ void add_scaled(f32x4 &acc, const f32x4 &part, float s) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] = fmaf(part[r], s, acc[r]);
+}
 // acc += sw * sa * (block of W) (block of A)^T; WB: the byte of sw that the scaled instruction takes
 template <bool E8M0, bool WIDE, int WB = 0, typename S>
 __device__ __forceinline__ void mma(const Frag<WIDE> &w, const Frag<WIDE> &a, f32x4 &acc, S sw, S sa) {
-    if constexpr (E8M0 && !WIDE) {
-        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, acc, 0, 0, WB, sw, 0, sa);
-    } else {
-        f32x4 part = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (WIDE) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) part = __builtin_amdgcn_mfma_f32_16x16x32_f16(w.v[i], a.v[i], part, 0, 0, 0);
-        } else part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, part, 0, 0, 0, 0, 0, 0);      // (unscaled)
-        const float s = sw * sa;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = fmaf(part[r], s, acc[r]);
-    }
+    if constexpr (E8M0 && !WIDE) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, acc, 0, 0, WB, sw, 0, sa);
+    else add_scaled(acc, product<WIDE>(w, a), sw * sa);
 }
 
 // act(v) + residual for CNT consecutive columns of one row, rounded once. FULL: all of them are inside; otherwise the first `left`.
@@ -342,6 +345,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
     for (int f = 0; f < FN; ++f) wraw[f] = read_w(0, f);
 #pragma unroll
     for (int j = 0; j < PD; ++j) araw[j] = read_a(0, j);
+    // parts that are scaled by the vector unit are added one product later: the matrix unit has the next one by then
+    constexpr bool BY_PART = !E8M0 || WIDE;
+    f32x4 late = {0.f, 0.f, 0.f, 0.f};
+    float late_scale = 0.f;
     // one block of K; S = kb % 4. No branches inside: the compiler would gather the products behind them. (A block behind the last one is filled
     // with zeros, its descriptor's range being empty, and read for nothing.)
     auto step = [&](int kb, auto s_) {
@@ -368,8 +375,14 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
             const auto sav = scale_of<E8M0, WIDE>(araw[j % SLOTS].scale);
 #pragma unroll
             for (int f = 0; f < FN; ++f) {
-                mma<E8M0, WIDE, S>(wf[f], af, acc[f][j], swv, sav);
-                if (!E8M0 || WIDE) asm volatile("" : "+v"(acc[f][j]));             // (the sum is made here: kept back, the parts would fill the registers)
+                if constexpr (BY_PART) {
+                    const f32x4 part = product<WIDE>(wf[f], af);
+                    __builtin_amdgcn_sched_barrier(0);
+                    f32x4 &to = f ? acc[f - 1][j] : j ? acc[FN - 1][j - 1] : acc[FN - 1][FM - 1];
+                    add_scaled(to, late, late_scale);
+                    asm volatile("" : "+v"(to));               // (the sum is made here: kept back, the parts would fill the registers)
+                    late = part, late_scale = swv * sav;
+                } else mma<E8M0, WIDE, S>(wf[f], af, acc[f][j], swv, sav);
                 if (j == FM - 1) {                             // this was the fragment's last use: the next block's takes its registers
                     __builtin_amdgcn_sched_barrier(0);
                     wraw[f] = read_w(kb + 1, f);
@@ -391,6 +404,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
         step(kb, std::integral_constant<int, 3>{});
         if (++kb == p.nkb) break;
     }
+
+    if constexpr (BY_PART) add_scaled(acc[FN - 1][FM - 1], late, late_scale);
 
     // Out through the LDS, 64 x 64 of a wave's tile at a time in a part of its own: whole 128- or 256-byte pieces of rows, and a short loop
     // instead of a long unrolled one (a tile's registers cannot be indexed; 16 KB of code cost more to fetch than the tile takes to store).
