@@ -12,7 +12,8 @@
 // fragment, and with the weight rows of a 64-column group dealt to the fragments as n = 16 * (r / 4) + 4 * f + r % 4 it holds 16
 // consecutive columns over four fragments: rows of y leave in 32- or 64-byte pieces. The order of k inside a block is free as long
 // as both operands share it: a lane's 32 bytes are the 16-byte chunks q and q + 4 (q = lane / 16).
-#include <cstdlib>
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include "rows.h"
 
@@ -464,6 +465,7 @@ template <int MF, int NF, bool E8M0, typename T> static int launch_direct(Matmul
     p.tiles_n = (p.N + 16 * NF - 1) / (16 * NF);
     const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
     LSSVC_CHECK(total < (1LL << 31), "matmul_fp8: %lld tiles do not fit one launch", (long long)total);
+    // (8 waves need 8 blocks each has one of; 16 waves are no faster at any size)
     return p.nkb <= 8 ? launch_direct<MF, NF, E8M0, T, 4>(p, total, s) : launch_direct<MF, NF, E8M0, T, 8>(p, total, s);
 }
 
@@ -479,24 +481,36 @@ template <int BM, int BN, int WM, int WN, bool E8M0, typename T> static int laun
     return launch_status("matmul_fp8");
 }
 
+// Which form: the one with the least estimated time, in us, from times measured at 26 sizes between 1 x 4096 x 4096 and 8192^3 (bf16, e8m0;
+// estimates are within 30 % of them). Direct: 3 us, what its workgroups read (6.5 MB a us if all CUs have one) and 0.25 us for every 256
+// workgroups. Tiles: a start, and for every tile that a CU gets its blocks of K and an end. Two rounds' worth of tiles cost two rounds: the
+// estimate is where the 256 x 256 form's half-empty last round is weighed against the smaller tiles' lower rate.
 template <bool E8M0, typename T> static int launch_matmul(const MatmulP &p, hipStream_t s) {
-    const int force = getenv("FP8_FORCE") ? atoi(getenv("FP8_FORCE")) : 0;
-    if (force) switch (force) {
-        case 11: return launch_direct<1, 1, E8M0, T>(p, s);
-        case 21: return launch_direct<2, 1, E8M0, T>(p, s);
-        case 41: return launch_direct<4, 1, E8M0, T>(p, s);
-        case 24: return launch_direct<2, 4, E8M0, T>(p, s);
-        case 44: return launch_direct<4, 4, E8M0, T>(p, s);
-        case 128: return launch_tile<128, 128, 64, 64, E8M0, T>(p, s);
-        case 256: if constexpr (sizeof(T) == 2) return launch_tile<256, 256, 128, 64, E8M0, T>(p, s); else return launch_tile<128, 128, 64, 64, E8M0, T>(p, s);
+    constexpr bool WIDE = sizeof(T) == 4;
+    auto tiles = [&](int bm, int bn) { return (double)((p.M + bm - 1) / bm) * (double)((p.N + bn - 1) / bn); };
+    auto direct = [&](int mf, int nf) {
+        const double t = tiles(16 * mf, 16 * nf);
+        return 3.0 + t * p.nkb * (mf + nf) * 2048 / (6.5e6 * std::min(1.0, t / 256)) + t / 1024;
+    };
+    auto tiled = [&](int bm, double start, double block, double end) { return start + std::ceil(tiles(bm, bm) / 256) * (p.nkb * block + end); };
+    // (a pitch that is no multiple of 128: a block of K straddles two lines)
+    const double rate = (WIDE ? 1.9 : E8M0 ? 1.0 : 1.17) * ((p.lda | p.ldw) % 128 && p.nkb > 1 ? 1.6 : 1.0);
+    const double cost[6] = {direct(1, 1), direct(1, 4), direct(2, 4), direct(4, 4), tiled(128, 4.5, 0.56 * rate, 1.0), WIDE ? 1e30 : tiled(256, 7.0, 1.42 * rate, 5.0)};
+#ifdef FP8_SWEEP
+    const int best = getenv("FP8_FORCE") && atoi(getenv("FP8_FORCE")) >= 0 ? atoi(getenv("FP8_FORCE")) : (int)(std::min_element(cost, cost + 6) - cost);
+#else
+    const int best = (int)(std::min_element(cost, cost + 6) - cost);
+#endif
+    switch (best) {
+        case 0: return launch_direct<1, 1, E8M0, T>(p, s);
+        case 1: return launch_direct<1, 4, E8M0, T>(p, s);
+        case 2: return launch_direct<2, 4, E8M0, T>(p, s);
+        case 3: return launch_direct<4, 4, E8M0, T>(p, s);
+        case 5:
+            if constexpr (!WIDE) return launch_tile<256, 256, 128, 64, E8M0, T>(p, s);
+            break;
     }
-    if (p.M <= 16) return launch_direct<1, 1, E8M0, T>(p, s);
-    if (p.M <= 32) return launch_direct<2, 1, E8M0, T>(p, s);
-    auto tiles = [&](int bm, int bn) { return (int64_t)((p.M + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-    if constexpr (sizeof(T) == 2)
-        if (tiles(256, 256) >= 200) return launch_tile<256, 256, 128, 64, E8M0, T>(p, s);
-    if (tiles(128, 128) >= 200) return launch_tile<128, 128, 64, 64, E8M0, T>(p, s);
-    return launch_direct<4, 4, E8M0, T>(p, s);
+    return launch_tile<128, 128, 64, 64, E8M0, T>(p, s);
 }
 template <bool E8M0> static int launch_typed(const MatmulP &p, hipStream_t s) {
     if (p.dtype == LSSVC_F32) return launch_matmul<E8M0, float>(p, s);

@@ -36,6 +36,7 @@ struct NormP {
     Act act;
     float eps;
     int in_place;                // y is x: a row's last thread stores its own channels only
+    int parts;                   // resident form: workgroups that share a slice's rows on the way out
     int nv;                      // threads of a row of a full slice; multiplications that divide by it, by a unit's width and by its share of a row
     uint32_t m_nv, m_uw, m_w;
 };
@@ -86,11 +87,12 @@ template <typename T, int V, bool NARROW = false> __device__ __forceinline__ Pac
 }
 
 // Sums over (rows in flight x channels) per unit: v[j] is the thread's sum for channel lo + j. Entries go to the LDS, each unit is added up
-// by 2^sh lanes of one wave (all 64 unless there are more units than waves) in a fixed order, four reads in flight, and `done` makes of each
+// by 2^sh lanes (of several waves where there are fewer units than waves) in a fixed order, four reads in flight, and `done` makes of each
 // total what comes back in `tot`. ONE: V divides the unit width, so a thread's channels lie in one unit and are added before.
 template <int TPB, int V, bool ONE, typename F>
 __device__ __forceinline__ void unit_sums(const float (&v)[V], const Lane<V> &l, int nv, int rp, int sc, int uw, uint32_t m_w, int nu, float *ebuf, float *tot, F done) {
     const int t = threadIdx.x;
+    __shared__ float wsum[TPB / 64];
     if (l.live) {
         if constexpr (ONE) {
             float s = 0.f;
@@ -105,7 +107,7 @@ __device__ __forceinline__ void unit_sums(const float (&v)[V], const Lane<V> &l,
     }
     __syncthreads();
     const int W = ONE ? uw / V : uw, pitch = ONE ? nv : sc;
-    int sh = 6;
+    int sh = TPB == 512 ? 9 : 8;
     while (sh > 0 && (nu << sh) > TPB) --sh;
     const int lpu = 1 << sh, li = t & (lpu - 1);
     const int dr = divided(lpu, m_w), dc = lpu - dr * W;
@@ -125,15 +127,26 @@ __device__ __forceinline__ void unit_sums(const float (&v)[V], const Lane<V> &l,
             }
         }
         float a = (s[0] + s[1]) + (s[2] + s[3]);
-        if (sh == 6) {
+        if (sh >= 6) {
             a = wave_sum_hi(a);
-            if (li == 63) tot[u] = done(u, a);
+            if ((t & 63) == 63) {
+                if (sh == 6) tot[u] = done(u, a);
+                else wsum[t >> 6] = a;
+            }
         } else {
             for (int o = lpu >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o);
             if (li == 0) tot[u] = done(u, a);
         }
     }
     __syncthreads();
+    if (sh > 6) {                                              // (then there are at most TPB / 128 units)
+        if (t < nu) {
+            float a = 0.f;
+            for (int w = 0; w < 1 << (sh - 6); ++w) a += wsum[(t << (sh - 6)) + w];
+            tot[t] = done(t, a);
+        }
+        __syncthreads();
+    }
 }
 
 template <typename T, int V, bool ONE>
@@ -374,6 +387,8 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int
 }
 
 // ---- resident form --------------------------------------------------------------------------------------------------------------------
+// Where there are few groups, several workgroups hold the same slice, make the same statistics of it and share its rows on the way out, which
+// is the longest part (and not possible where x is written over).
 // Rolled loops on purpose: the form serves small maps, whose time is latency, and 50 KB of straight-line code cost more to fetch than the map
 // (27 us for 3 x 1961 x 100 fp16 with the slice in registers and everything unrolled).
 template <typename T, int V, int TPB, bool ONE, bool TO8>
@@ -382,7 +397,10 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
     using D = Pack<T, V>;
     using W = std::conditional_t<(sizeof(D) >= 16), i32x4, T>;  // how a thread's data lies in the LDS
     extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
-    const int sl = blockIdx.x % (unsigned)p.nslices, img = blockIdx.x / (unsigned)p.nslices, t = threadIdx.x;
+    unsigned id = blockIdx.x;
+    const int part = id % (unsigned)p.parts;
+    id /= (unsigned)p.parts;
+    const int sl = id % (unsigned)p.nslices, img = id / (unsigned)p.nslices, t = threadIdx.x;
     const int s0 = sl * p.slice, sc = min(p.slice, p.C - s0), uw = p.cg, mu = divided(p.slice, p.m_uw), nu = divided(sc, p.m_uw);
     float *ebuf = (float *)dyn, *umean = ebuf + TPB * (ONE ? 1 : V), *urstd = umean + mu, *piv = urstd + mu;
     constexpr int Q = sizeof(D) / sizeof(W);
@@ -460,9 +478,11 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
     if (!l.live) return;
 #pragma unroll
     for (int j = 0; j < V; ++j) f.a[j] *= urstd[un[j]];
-    at = data;
-    int64_t row = (int64_t)img * R + l.rt;
-    for (int r = l.rt; r < R; r += rp, at += Q * TPB, row += rp) {     // (the 16 lanes of a block share r)
+    // this workgroup's share of the rows
+    const int its = (R + rp - 1) / rp, share = (its + p.parts - 1) / p.parts, from = part * share, end = min(R, (from + share) * rp);
+    at = data + from * (Q * TPB);
+    int64_t row = (int64_t)img * R + l.rt + from * rp;
+    for (int r = l.rt + from * rp; r < end; r += rp, at += Q * TPB, row += rp) {     // (the 16 lanes of a block share r)
         float y[V];
         finish<T, V>(get(at), f, p, y);
         if constexpr (TO8) store_lane_fp8(p.q + row * p.ldq + s0, p.qs + row * p.ldqs + s0 / kFp8Block, l, sc, y);
@@ -535,9 +555,11 @@ template <typename T, int V, int TPB, bool ONE, bool TO8> static int launch_resi
     static LdsGrant grant;
     if (int rc = grant.ensure((const void *)norm_resident_kernel<T, V, TPB, ONE, TO8>, q.lds, 64 * 1024)) return rc;
     NormP n = p;
+    const int rp = TPB / threads_of<V, TO8>(q.slice), its = (int)((p.R + rp - 1) / rp);
+    n.parts = p.in_place ? 1 : std::max(1, std::min(std::min(8, (its + 1) / 2), 256 / std::min(256, images * q.nslices)));
     n.nv = threads_of<V, TO8>(q.slice), n.m_nv = division_magic(n.nv);
     n.m_uw = division_magic(p.cg), n.m_w = division_magic(ONE ? p.cg / V : p.cg);
-    norm_resident_kernel<T, V, TPB, ONE, TO8><<<(unsigned)(images * q.nslices), TPB, q.lds, s>>>(n);
+    norm_resident_kernel<T, V, TPB, ONE, TO8><<<(unsigned)(images * q.nslices * n.parts), TPB, q.lds, s>>>(n);
     return launch_status("group_norm");
 }
 template <typename T, int TPB> static int launch_resident(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {

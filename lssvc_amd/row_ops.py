@@ -120,10 +120,10 @@ class Fp8Rows:
             _refuse("Fp8Rows: scale is %s, expected %s for %d x %d values in %d x %d blocks", tuple(scale.shape), want, rows, cols, block_rows, BLOCK)
         _no_grad(scale, "scale")
         if rows and not (cols % 16 == 0 and values.stride(1) == 1 and (rows == 1 or values.stride(0) % 16 == 0 and values.stride(0) >= cols) and values.data_ptr() % 16 == 0):
-            values = _padded(values, 16)
+            values = _padded(values, _pitch(cols))
         if rows and scale.dtype == _E8M0 and not (want[1] % 4 == 0 and scale.stride(1) == 1 and scale.data_ptr() % 4 == 0
                                                   and (want[0] == 1 or scale.stride(0) % 4 == 0 and scale.stride(0) >= want[1])):
-            scale = _padded(scale, 4)
+            scale = _padded(scale, -(-want[1] // 4) * 4)
         elif rows and scale.dtype == torch.float32 and not ((scale.stride(1) == 1 or want[1] == 1) and (want[0] == 1 or scale.stride(0) >= want[1])):
             scale = scale.contiguous()
         self._set(values, scale, block_rows)
@@ -133,7 +133,7 @@ class Fp8Rows:
         kb = -(-cols // BLOCK)
         self._values, self._scale, self.rows, self.cols, self.block_rows, self.device = values, scale, rows, cols, block_rows, values.device
         e8m0 = scale.dtype == _E8M0
-        ld = values.stride(0) if rows > 1 else -(-cols // 16) * 16
+        ld = values.stride(0) if rows > 1 else _pitch(cols)
         sld = scale.stride(0) if scale.shape[0] > 1 else (-(-kb // 4) * 4 if e8m0 else kb)
         self._c = Fp8(values.data_ptr(), scale.data_ptr(), rows, ld, sld, cols, block_rows, 1 if e8m0 else 0, 0)
         self._store = None
@@ -158,7 +158,7 @@ class Fp8Rows:
             _refuse("Fp8Rows: block_rows is 1 or %d, got %r", BLOCK, block_rows)
         if rows < 0 or cols < 1:
             _refuse("Fp8Rows: %d x %d values", rows, cols)
-        ld, sld = -(-cols // 16) * 16, -(-cols // (4 * BLOCK)) * 4
+        ld, sld = _pitch(cols), -(-cols // (4 * BLOCK)) * 4
         nbytes = rows * ld
         self = Fp8Rows.__new__(Fp8Rows)
         self._store = store = torch.empty(nbytes + -(-rows // block_rows) * sld, dtype=torch.uint8, device=device)
@@ -176,9 +176,15 @@ class Fp8Rows:
         return (self.values.float() * s).to(dtype)
 
 
-def _padded(x, to):
-    """A copy of 8-bit rows in a buffer whose pitch is the next multiple of `to` bytes, zeros behind the last column."""
-    store = torch.zeros(x.shape[0], -(-x.shape[1] // to) * to, dtype=torch.uint8, device=x.device)
+def _pitch(cols):
+    """Bytes between rows of 8-bit values: whole 128-byte lines per block of K (a block that straddles two lines costs the product up to
+    1.9x: 1362 x 553 x 5993 44 us at a pitch of 6000, 25 us at 6016); short rows stay close together."""
+    return -(-cols // 16) * 16 if cols <= BLOCK else -(-cols // BLOCK) * BLOCK
+
+
+def _padded(x, pitch):
+    """A copy of 8-bit rows in a buffer with `pitch` bytes between rows, zeros behind the last column."""
+    store = torch.zeros(x.shape[0], pitch, dtype=torch.uint8, device=x.device)
     store[:, :x.shape[1]] = x.contiguous().view(torch.uint8)
     return store.view(x.dtype)[:, :x.shape[1]]
 

@@ -113,9 +113,9 @@ def check_fp8(q, want, tol):
 
 def behind(q):
     """The bytes of each row from the last column to the next multiple of 16."""
-    ld = -(-q.cols // 16) * 16
-    assert q.values.stride(0) == ld and q.values.data_ptr() % 16 == 0
-    return q.values.as_strided((q.rows, ld), (ld, 1)).view(torch.uint8)[:, q.cols:]
+    ld = q.values.stride(0)
+    assert ld % 16 == 0 and q.values.data_ptr() % 16 == 0
+    return q.values.as_strided((q.rows, -(-q.cols // 16) * 16), (ld, 1)).view(torch.uint8)[:, q.cols:]
 
 
 @pytest.mark.parametrize("offset", [100.0, 3000.0])
