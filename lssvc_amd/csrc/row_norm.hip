@@ -3,12 +3,13 @@
 // y = act((x - mu) * rsqrt(var + eps) * w_c + b_c), mu / var over the rows of an image and the cg = C / G channels of a group. The
 // operator is bound by memory: one read and one write of the map if it stays on the chip between the statistics and their use, two reads
 // otherwise. Two forms:
-//   resident  a workgroup owns all rows of a slice of whole groups and holds the slice in the LDS (up to 128 KB; every thread reads back
+//   resident  a workgroup owns all rows of a slice of whole groups and holds the slice in the LDS (up to 159 KB; every thread reads back
 //             what it wrote itself): one read, one write, one launch.
 //   split     rows are split over workgroups that write (mean, M2) per chunk and group; one wave per group merges the chunks; the
 //             normalising pass reads the map again, in the opposite order, so that what the first pass read last comes from the caches.
-// Every sum is taken of differences to a value of the group itself (a pivot), and squares of differences to a mean, never E[x^2] - E[x]^2:
-// a map whose offset is a thousand times its spread keeps the digits of its spread.
+// A thread makes (mean, M2) of what it reads, of differences to a value of its own (its share of the squares cannot be lost in them: the
+// value is one of the data), in fp32; from there on sums S1 = sum x and S2 = sum x^2 are in 64 bits, where S2 - S1^2 / N keeps what fp32
+// data can hold: an offset a thousand times the spread costs 2^-33 of the variance.
 //
 // One thread handles V consecutive channels: 16 bytes at any alignment (8 channels where 8-bit blocks are written). Where V does not divide
 // the slice, a row's last thread loads the LAST V channels -- wide loads only -- and owns those that its neighbour does not (a slice of fewer
@@ -27,7 +28,8 @@ struct NormP {
     int64_t ldx, ldy, ldq, ldqs;
     int64_t R;                   // rows of an image
     const float *w, *b;
-    float2 *part, *stat;         // split form: [image][chunk][unit] (mean, M2); [image][channel] (mean, weight / sqrt(var + eps))
+    double2 *part;               // split form: [image][chunk][unit] (S1, S2)
+    float2 *stat;                // split form: [image][channel] (mean, weight / sqrt(var + eps))
     int64_t chunk;               // rows of a chunk
     int C, G, cg;
     int S;                       // chunks of an image
@@ -73,6 +75,9 @@ template <int V> struct Lane {
     }
 };
 
+// quotients of uniform values, once per workgroup
+__device__ __forceinline__ int divided_any(int a, int b) { return (int)((unsigned)a / (unsigned)b); }
+
 // threads of a row that is `sc` columns wide (the 8-bit form: 16 for every block of 128)
 template <int V, bool TO8> __host__ __device__ __forceinline__ int threads_of(int sc) {
     return TO8 ? (sc + kFp8Block - 1) / kFp8Block * (kFp8Block / 8) : (sc + V - 1) / V;
@@ -86,74 +91,87 @@ template <typename T, int V, bool NARROW = false> __device__ __forceinline__ Pac
     return r;
 }
 
-// Sums over (rows in flight x channels) per unit: v[j] is the thread's sum for channel lo + j. Entries go to the LDS, each unit is added up
-// by 2^sh lanes (of several waves where there are fewer units than waves) in a fixed order, four reads in flight, and `done` makes of each
-// total what comes back in `tot`. ONE: V divides the unit width, so a thread's channels lie in one unit and are added before.
+// (S1, S2) of every unit of a slice from the threads' (mean, M2) of n rows each: entries go to the LDS, a unit's are added up by 2^sh lanes
+// (of several waves where there are fewer units than waves) in a fixed order, and one lane hands the totals to `done`. ONE: V divides the
+// unit width, a thread's channels lie in one unit and are added before. A thread's n is `q` or, for the first `rem` rows in flight, q + 1.
+template <int TPB, int V, bool ONE> constexpr int kEntryBytes = ONE ? TPB * 16 : TPB * V * 8;
 template <int TPB, int V, bool ONE, typename F>
-__device__ __forceinline__ void unit_sums(const float (&v)[V], const Lane<V> &l, int nv, int rp, int sc, int uw, uint32_t m_w, int nu, float *ebuf, float *tot, F done) {
+__device__ __forceinline__ void unit_sums(const float (&mean)[V], const float (&m2)[V], int q, int rem, const Lane<V> &l, int nv, int rp, int sc, int uw, uint32_t m_w,
+                                          int nu, void *entries, F done) {
     const int t = threadIdx.x;
-    __shared__ float wsum[TPB / 64];
+    __shared__ double2 wsum[TPB / 64];
+    double2 *one = (double2 *)entries;
+    float2 *each = (float2 *)entries;
     if (l.live) {
         if constexpr (ONE) {
-            float s = 0.f;
+            const double n = q + (l.rt < rem ? 1 : 0);
+            double a = 0, b = 0;
+            float m = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; ++j) s += v[j];
-            ebuf[l.rt * nv + l.cv] = s;
+            for (int j = 0; j < V; ++j) a += mean[j], b = fma((double)mean[j], (double)mean[j], b), m += m2[j];
+            one[l.rt * nv + l.cv] = n > 0 ? make_double2(n * a, fma(n, b, (double)m)) : make_double2(0, 0);
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (l.owns(j)) ebuf[l.rt * sc + l.lo + j] = v[j];
+                if (l.owns(j)) each[l.rt * sc + l.lo + j] = make_float2(mean[j], m2[j]);
         }
     }
     __syncthreads();
     const int W = ONE ? uw / V : uw, pitch = ONE ? nv : sc;
+    const int live_rows = q > 0 ? rp : rem;                    // rows in flight that hold anything
     int sh = TPB == 512 ? 9 : 8;
     while (sh > 0 && (nu << sh) > TPB) --sh;
     const int lpu = 1 << sh, li = t & (lpu - 1);
     const int dr = divided(lpu, m_w), dc = lpu - dr * W;
-    const int r0 = divided(li, m_w), c0 = li - r0 * W;
+    int r = divided(li, m_w), c = li - r * W;
+    const int r0 = r, c0 = c;
     for (int u = t >> sh; u < nu; u += TPB >> sh) {
-        float s[4] = {};
-        int r = r0, c = c0;
-        while (r < rp) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const bool on = r < rp;
-                const float x = ebuf[on ? r * pitch + u * W + c : 0];
-                s[k] += on ? x : 0.f;
-                r += dr;
-                c += dc;
-                if (c >= W) c -= W, ++r;
+        double a = 0, b = 0;
+        r = r0, c = c0;
+#pragma unroll 2
+        while (r < live_rows) {
+            const int at = r * pitch + u * W + c;
+            if constexpr (ONE) a += one[at].x, b += one[at].y;
+            else {
+                const float2 e = each[at];
+                const double n = q + (r < rem ? 1 : 0), m = e.x;
+                a = fma(n, m, a);
+                b += fma(n * m, m, (double)e.y);
             }
+            r += dr;
+            c += dc;
+            if (c >= W) c -= W, ++r;
         }
-        float a = (s[0] + s[1]) + (s[2] + s[3]);
         if (sh >= 6) {
-            a = wave_sum_hi(a);
+            a = wave_sum_hi(a), b = wave_sum_hi(b);
             if ((t & 63) == 63) {
-                if (sh == 6) tot[u] = done(u, a);
-                else wsum[t >> 6] = a;
+                if (sh == 6) done(u, a, b);
+                else wsum[t >> 6] = make_double2(a, b);
             }
         } else {
-            for (int o = lpu >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o);
-            if (li == 0) tot[u] = done(u, a);
+            for (int o = lpu >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o), b += __shfl_xor(b, o);
+            if (li == 0) done(u, a, b);
         }
     }
-    __syncthreads();
     if (sh > 6) {                                              // (then there are at most TPB / 128 units)
-        if (t < nu) {
-            float a = 0.f;
-            for (int w = 0; w < 1 << (sh - 6); ++w) a += wsum[(t << (sh - 6)) + w];
-            tot[t] = done(t, a);
-        }
         __syncthreads();
+        if (t < nu) {
+            double a = 0, b = 0;
+            for (int w = 0; w < 1 << (sh - 6); ++w) a += wsum[(t << (sh - 6)) + w].x, b += wsum[(t << (sh - 6)) + w].y;
+            done(t, a, b);
+        }
     }
 }
+__device__ __forceinline__ float2 moments(double s1, double s2, double n, float eps) {       // (mean, 1 / sqrt(var + eps))
+    const double mean = s1 / n, var = s2 / n - mean * mean;
+    return make_float2((float)mean, 1.f / sqrtf((var < 0 ? 0.f : (float)var) + eps));         // (NaN stays NaN)
+}
 
+// ---- split form, first pass: (S1, S2) of each chunk and unit -----------------------------------------------------------------------
 template <typename T, int V, bool ONE>
 __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
     constexpr int TPB = 256, NB = 4;
-    __shared__ float ebuf[ONE ? TPB : TPB * V];
-    __shared__ float tot[kSliceMax], piv[kSliceMax], umean[kSliceMax];
+    __shared__ __attribute__((aligned(16))) uint8_t entries[kEntryBytes<TPB, V, ONE>];
     unsigned id = blockIdx.x;
     const int sl = id % (unsigned)p.nslices;
     id /= (unsigned)p.nslices;
@@ -163,7 +181,7 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
         s0 = sl * p.slice;
         sc = min(p.slice, p.C - s0);
         uw = p.cg;
-        nu = sc / uw;
+        nu = divided(sc, p.m_uw);
     } else {
         const int g = sl / p.P, k = sl - g * p.P;
         s0 = g * p.cg + k * p.piece;
@@ -171,15 +189,16 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
         nu = 1;
     }
     int nv = p.nv;
-    uint32_t m_nv = p.m_nv, m_uw = p.m_uw, m_w = p.m_w;
-    if (sc != p.slice) nv = (sc + V - 1) / V, m_nv = division_magic(nv);           // the last slice; the last piece of a group
-    if (p.P > 1 && sc != p.slice) m_uw = division_magic(uw), m_w = division_magic(ONE ? uw / V : uw);
+    uint32_t m_nv = p.m_nv, m_w = p.m_w;
+    if (sc != p.slice) {                                       // the last slice; the last piece of a group
+        nv = (sc + V - 1) / V, m_nv = division_magic(nv);
+        if (p.P > 1) m_w = division_magic(ONE ? uw / V : uw);
+    }
     const int rp = divided(TPB, m_nv), t = threadIdx.x;
     const Lane<V> l(t, nv, m_nv, rp, sc);
     const int64_t r0 = chunk * p.chunk, r1 = min(r0 + p.chunk, p.R);
     const T *base = (const T *)p.x + ((int64_t)img * p.R + r0) * p.ldx + s0;
     const int rows = (int)(r1 - r0);
-    for (int u = t; u < nu; u += TPB) piv[u] = to_f32(base[u * uw]);
 
     float n = 0.f, mean[V] = {}, m2[V] = {};
     if (l.live) {
@@ -224,67 +243,31 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
             n += 1.f;
         }
     }
-    __syncthreads();             // piv
-    float v[V];
-    int un[V];
-    l.template units<ONE>(uw, m_uw, nu, un);
-#pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = n == 0.f ? 0.f : n * (mean[j] - piv[un[j]]);
-    const float inv = 1.f / ((float)rows * (float)uw);
-    unit_sums<TPB, V, ONE>(v, l, nv, rp, sc, uw, m_w, nu, ebuf, umean, [&](int u, float s) { return fmaf(s, inv, piv[u]); });
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float d = mean[j] - umean[un[j]];
-        v[j] = n == 0.f ? 0.f : fmaf(n * d, d, m2[j]);
-    }
-    unit_sums<TPB, V, ONE>(v, l, nv, rp, sc, uw, m_w, nu, ebuf, tot, [](int, float s) { return s; });
-    const int U = p.G * p.P, u0 = p.P == 1 ? s0 / p.cg : sl;
-    float2 *out = p.part + ((int64_t)img * p.S + chunk) * U + u0;
-    for (int u = t; u < nu; u += TPB) out[u] = make_float2(umean[u], tot[u]);
+    const int per = divided_any(rows, rp), rem = rows - per * rp;
+    double2 *out = p.part + ((int64_t)img * p.S + chunk) * (p.G * p.P) + (p.P == 1 ? divided_any(s0, p.cg) : sl);
+    unit_sums<TPB, V, ONE>(mean, m2, per, rem, l, nv, rp, sc, uw, m_w, nu, entries, [&](int u, double a, double b) { out[u] = make_double2(a, b); });
 }
 
-// ---- split form, merge: a workgroup per image and group joins the chunks and writes (mean, weight / sqrt(var + eps)) of its channels -------
-// The chunks' statistics are read once, all loads on their way together (a chain of dependent reads is what this small kernel would cost).
+// ---- split form, merge: a workgroup per image and group adds up the chunks and writes (mean, weight / sqrt(var + eps)) of its channels -----
 __global__ __launch_bounds__(256) void norm_merge_kernel(NormP p) {
-    constexpr int E = 8;                                        // entries per thread in registers: host keeps S * P <= 256 * E
-    __shared__ float red[2][4];
+    __shared__ double2 red[4];
     const int img = blockIdx.x / (unsigned)p.G, g = blockIdx.x - img * p.G, t = threadIdx.x;
     const int U = p.G * p.P, n = p.S * p.P;
-    const float2 *src = p.part + (int64_t)img * p.S * U + g * p.P;
-    const float pivot = src[0].x, inv = 1.f / ((float)p.R * (float)p.cg);
-    float2 v[E];
-    float w[E], s = 0.f;
-#pragma unroll
-    for (int k = 0; k < E; ++k) {
-        const int e = t + 256 * k;
-        w[k] = 0.f, v[k] = make_float2(0.f, 0.f);
-        if (e < n) {
-            const int c = p.P == 1 ? e : e / p.P, i = e - c * p.P;
-            v[k] = src[(int64_t)c * U + i];
-            w[k] = (float)min(p.chunk, p.R - (int64_t)c * p.chunk) * (float)(p.P == 1 ? p.cg : min(p.piece, p.cg - i * p.piece));
-        }
+    const double2 *src = p.part + (int64_t)img * p.S * U + g * p.P;
+    double a = 0, b = 0;
+#pragma unroll 4
+    for (int e = t; e < n; e += 256) {
+        const int c = p.P == 1 ? e : e / p.P;
+        const double2 v = src[(int64_t)c * U + (e - c * p.P)];
+        a += v.x, b += v.y;
     }
-#pragma unroll
-    for (int k = 0; k < E; ++k)
-        if (w[k] != 0.f) s = fmaf(w[k], v[k].x - pivot, s);
-    s = wave_sum_hi(s);
-    if ((t & 63) == 63) red[0][t >> 6] = s;
+    a = wave_sum_hi(a), b = wave_sum_hi(b);
+    if ((t & 63) == 63) red[t >> 6] = make_double2(a, b);
     __syncthreads();
-    const float mean = fmaf((red[0][0] + red[0][1]) + (red[0][2] + red[0][3]), inv, pivot);
-    s = 0.f;
-#pragma unroll
-    for (int k = 0; k < E; ++k)
-        if (w[k] != 0.f) {
-            const float d = v[k].x - mean;
-            s += fmaf(w[k] * d, d, v[k].y);
-        }
-    s = wave_sum_hi(s);
-    if ((t & 63) == 63) red[1][t >> 6] = s;
-    __syncthreads();
-    const float rstd = 1.f / sqrtf(fmaf((red[1][0] + red[1][1]) + (red[1][2] + red[1][3]), inv, p.eps));
+    const float2 m = moments((red[0].x + red[1].x) + (red[2].x + red[3].x), (red[0].y + red[1].y) + (red[2].y + red[3].y), (double)p.R * p.cg, p.eps);
     float2 *out = p.stat + (int64_t)img * p.C + g * p.cg;
     const float *wt = p.w ? p.w + g * p.cg : nullptr;
-    for (int c = t; c < p.cg; c += 256) out[c] = make_float2(mean, wt ? rstd * wt[c] : rstd);
+    for (int c = t; c < p.cg; c += 256) out[c] = make_float2(m.x, wt ? m.y * wt[c] : m.y);
 }
 
 // ---- normalise, activate, store: shared by both forms -------------------------------------------------------------------------------
@@ -402,9 +385,9 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
     id /= (unsigned)p.parts;
     const int sl = id % (unsigned)p.nslices, img = id / (unsigned)p.nslices, t = threadIdx.x;
     const int s0 = sl * p.slice, sc = min(p.slice, p.C - s0), uw = p.cg, mu = divided(p.slice, p.m_uw), nu = divided(sc, p.m_uw);
-    float *ebuf = (float *)dyn, *umean = ebuf + TPB * (ONE ? 1 : V), *urstd = umean + mu, *piv = urstd + mu;
+    float2 *stat = (float2 *)(dyn + kEntryBytes<TPB, V, ONE>);
     constexpr int Q = sizeof(D) / sizeof(W);
-    W *data = (W *)(dyn + (4 * (TPB * (ONE ? 1 : V) + 3 * mu) + 15) / 16 * 16) + t;
+    W *data = (W *)(dyn + kEntryBytes<TPB, V, ONE> + (8 * mu + 15) / 16 * 16) + t;
     auto put = [&](W *to, const D &x) {
         W v[Q];
         __builtin_memcpy(v, &x, sizeof(x));
@@ -432,7 +415,6 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
         for (int k = 0; k < NB; ++k) d[k] = load_lane<T, V, TO8>(base + (int64_t)min(r + k * rp, R - 1) * p.ldx, l);
     };
     load(l.rt);
-    for (int u = t; u < nu; u += TPB) piv[u] = to_f32(base[u * uw]);
     Affine<V> f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -440,12 +422,10 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
         f.a[j] = p.w ? p.w[c] : 1.f;
         f.b[j] = p.b ? p.b[c] : 0.f;
     }
-    int un[V];
-    l.template units<ONE>(uw, p.m_uw, nu, un);
-    __syncthreads();
-    float v[V] = {};
+    // sums of differences to the thread's first row
+    float x0[V], v1[V] = {}, v2[V] = {};
 #pragma unroll
-    for (int j = 0; j < V; ++j) f.mean[j] = piv[un[j]];
+    for (int j = 0; j < V; ++j) x0[j] = to_f32(d[0].v[j]);
     W *at = data;
     for (int r = l.rt; r < R;) {
 #pragma unroll
@@ -453,33 +433,38 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
             put(at + k * Q * TPB, d[k]);
             const bool on = r + k * rp < R;
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] += on ? to_f32(d[k].v[j]) - f.mean[j] : 0.f;
+            for (int j = 0; j < V; ++j) {
+                const float e = on ? to_f32(d[k].v[j]) - x0[j] : 0.f;
+                v1[j] += e;
+                v2[j] = fmaf(e, e, v2[j]);
+            }
         }
         at += NB * Q * TPB;
         r += NB * rp;
         if (r < R) load(r);
     }
-    const float inv = 1.f / ((float)R * (float)uw);
+    const int per = divided_any(R, rp), rem = R - per * rp;
+    const float n = per + (l.rt < rem ? 1 : 0), inv = n > 0.f ? 1.f / n : 0.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float m = v1[j] * inv;
+        v2[j] = fmaf(-v1[j], m, v2[j]);
+        v1[j] = x0[j] + m;
+    }
     Lane<V> le = l;                                            // (the 8-bit form's padding lanes own nothing and take no part in the sums)
     le.live = l.live && l.cv * V < sc;
-    unit_sums<TPB, V, ONE>(v, le, nv, rp, sc, uw, p.m_w, nu, ebuf, umean, [&](int u, float s) { return fmaf(s, inv, piv[u]); });
-#pragma unroll
-    for (int j = 0; j < V; ++j) f.mean[j] = umean[un[j]], v[j] = 0.f;
-    at = data;
-    for (int r = l.rt; r < R; r += rp, at += Q * TPB) {
-        const D x = get(at);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const float e = to_f32(x.v[j]) - f.mean[j];
-            v[j] = fmaf(e, e, v[j]);
-        }
-    }
-    unit_sums<TPB, V, ONE>(v, le, nv, rp, sc, uw, p.m_w, nu, ebuf, urstd, [&](int, float s) { return 1.f / sqrtf(fmaf(s, inv, p.eps)); });
+    unit_sums<TPB, V, ONE>(v1, v2, per, rem, le, nv, rp, sc, uw, p.m_w, nu, dyn, [&](int u, double a, double b) { stat[u] = moments(a, b, (double)R * uw, p.eps); });
+    __syncthreads();
     if (!l.live) return;
+    int un[V];
+    l.template units<ONE>(uw, p.m_uw, nu, un);
 #pragma unroll
-    for (int j = 0; j < V; ++j) f.a[j] *= urstd[un[j]];
+    for (int j = 0; j < V; ++j) {
+        const float2 s = stat[un[j]];
+        f.mean[j] = s.x, f.a[j] *= s.y;
+    }
     // this workgroup's share of the rows
-    const int its = (R + rp - 1) / rp, share = (its + p.parts - 1) / p.parts, from = part * share, end = min(R, (from + share) * rp);
+    const int its = per + (rem ? 1 : 0), share = (its + p.parts - 1) / p.parts, from = part * share, end = min(R, (from + share) * rp);
     at = data + from * (Q * TPB);
     int64_t row = (int64_t)img * R + l.rt + from * rp;
     for (int r = l.rt + from * rp; r < end; r += rp, at += Q * TPB, row += rp) {     // (the 16 lanes of a block share r)
@@ -501,8 +486,8 @@ struct NormPlan {
     bool one;
 };
 static int gcd_i(int a, int b) { return b ? gcd_i(b, a % b) : a; }
-constexpr int kMergeMax = 2048;          // chunks x pieces that the merge holds in registers
-constexpr int kResidentBytes = 128 * 1024;
+constexpr int kMergeMax = 2048;          // chunks x pieces: what one merging workgroup adds up
+constexpr int kResidentBytes = 159 * 1024;   // of the CU's 160 KB (a workgroup's own 128 bytes beside)
 
 static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8) {
     NormPlan q{};
@@ -522,8 +507,8 @@ static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8)
         q.tpb = nv <= 256 && R <= 8 * (256 / nv) ? 256 : 512;
         const int64_t rp = q.tpb / nv, its = (R + 4 * rp - 1) / (4 * rp) * 4;
         q.slice = (int)slice;
-        q.lds = (4 * (size_t)(q.tpb * (q.one ? 1 : V) + 3 * (slice / cg)) + 15) / 16 * 16 + (size_t)(its * q.tpb * V * es);
-        if (q.lds <= kResidentBytes + 16 * 1024) {
+        q.lds = (size_t)q.tpb * (q.one ? 16 : 8 * V) + (8 * (size_t)(slice / cg) + 15) / 16 * 16 + (size_t)(its * q.tpb * V * es);
+        if (q.lds <= kResidentBytes) {
             q.resident = true;
             q.nslices = (int)((C + slice - 1) / slice);
             return q;
@@ -548,7 +533,7 @@ static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8)
 }
 
 static int64_t norm_ws(const NormPlan &q, int images, int C, int G) {
-    return q.resident ? 0 : 8 * ((int64_t)images * q.S * G * q.P + (int64_t)images * C);
+    return q.resident ? 0 : 16 * (int64_t)images * q.S * G * q.P + 8 * (int64_t)images * C;
 }
 
 template <typename T, int V, int TPB, bool ONE, bool TO8> static int launch_resident(const NormP &p, const NormPlan &q, int images, hipStream_t s) {
@@ -657,8 +642,8 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     p.S = q.S, p.P = q.P, p.piece = q.piece, p.chunk = q.chunk, p.slice = q.slice, p.nslices = q.nslices;
     p.act = Act{act, slope}, p.eps = eps;
     p.in_place = y && y->ptr == x->ptr;
-    p.stat = (float2 *)workspace;
-    p.part = p.stat + (int64_t)images * x->cols;
+    p.part = (double2 *)workspace;
+    p.stat = (float2 *)(p.part + (int64_t)images * q.S * groups * q.P);
     hipStream_t s = (hipStream_t)stream;
     if (x->dtype == LSSVC_F32) return launch_norm<float>(p, q, images, y8 != nullptr, s);
     if (x->dtype == LSSVC_F16) return launch_norm<f16_t>(p, q, images, y8 != nullptr, s);

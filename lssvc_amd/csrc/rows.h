@@ -118,15 +118,19 @@ __device__ __forceinline__ uint32_t row16_finite_max(const float (&z)[8]) {
     return m;
 }
 // sum over the wave in a fixed order, valid in lane 63
-__device__ __forceinline__ float wave_sum_hi(float v) {
-#define LSSVC_DPP_ADD(ctrl, rows) v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), ctrl, rows, 0xf, false))
-    LSSVC_DPP_ADD(0x111, 0xf);               // row_shr:1, 2, 4, 8: lane 15 of each row has the row's sum
-    LSSVC_DPP_ADD(0x112, 0xf);
-    LSSVC_DPP_ADD(0x114, 0xf);
-    LSSVC_DPP_ADD(0x118, 0xf);
-    LSSVC_DPP_ADD(0x142, 0xa);               // row_bcast:15 into rows 1 and 3
-    LSSVC_DPP_ADD(0x143, 0xc);               // row_bcast:31 into rows 2 and 3
-#undef LSSVC_DPP_ADD
+template <int CTRL, int ROWS> __device__ __forceinline__ double dpp_move(double v) {      // lanes that get nothing get 0
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_sum_hi(double v) {
+    v += dpp_move<0x111, 0xf>(v);            // row_shr:1, 2, 4, 8: lane 15 of each row has the row's sum
+    v += dpp_move<0x112, 0xf>(v);
+    v += dpp_move<0x114, 0xf>(v);
+    v += dpp_move<0x118, 0xf>(v);
+    v += dpp_move<0x142, 0xa>(v);            // row_bcast:15 into rows 1 and 3
+    v += dpp_move<0x143, 0xc>(v);            // row_bcast:31 into rows 2 and 3
     return v;
 }
 // t / n for t < 2^16 and n < 2^16: one multiplication; magic = division_magic(n)
