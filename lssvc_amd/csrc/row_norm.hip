@@ -5,8 +5,9 @@
 // otherwise. Two forms:
 //   resident  a workgroup owns all rows of a slice of whole groups and holds the slice in the LDS (up to 159 KB; every thread reads back
 //             what it wrote itself): one read, one write, one launch.
-//   split     rows are split over workgroups that write (mean, M2) per chunk and group; one wave per group merges the chunks; the
-//             normalising pass reads the map again, in the opposite order, so that what the first pass read last comes from the caches.
+//   split     rows are split over workgroups that write sums per chunk and group; the chunks are joined by a launch of their own, or, where
+//             they are few, by every workgroup of the normalising pass for itself; that pass reads the map again, in the opposite order,
+//             so that what the first pass read last comes from the caches.
 // A thread makes (mean, M2) of what it reads, of differences to a value of its own (its share of the squares cannot be lost in them: the
 // value is one of the data), in fp32; from there on sums S1 = sum x and S2 = sum x^2 are in 64 bits, where S2 - S1^2 / N keeps what fp32
 // data can hold: an offset a thousand times the spread costs 2^-33 of the variance.
@@ -321,7 +322,8 @@ __device__ __forceinline__ void store_lane_fp8(uint8_t *qrow, uint8_t *srow, con
     if ((l.cv & 15) == 0) srow[l.cv >> 4] = (uint8_t)byte;
 }
 
-template <typename T, int V, bool TO8>
+// JOIN: (mean, 1 / sqrt(var + eps)) of the slice's groups from the chunks' sums, here
+template <typename T, int V, bool TO8, bool JOIN>
 __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int nsl, int S2, int64_t chunk2) {
     constexpr int TPB = 256, NB = TO8 ? 2 : 4;
     unsigned id = gridDim.x - 1 - blockIdx.x;                  // the opposite order of the first pass
@@ -334,6 +336,27 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int
     if (sc != width) nv = threads_of<V, TO8>(sc), m_nv = division_magic(nv);
     const int rp = divided(TPB, m_nv);
     const Lane<V> l(t, nv, m_nv, rp, sc);
+    __shared__ float2 joined[JOIN ? kSliceMax : 1];
+    const int first = JOIN ? divided_any(s0, p.cg) : 0;        // the slice's first group
+    if constexpr (JOIN) {
+        const int ng = divided_any(s0 + sc - 1, p.cg) - first + 1, U = p.G * p.P, n = p.S * p.P;
+        int sh = 6;
+        while (sh > 0 && (ng << sh) > TPB) --sh;
+        const int lanes = 1 << sh, li = t & (lanes - 1);
+        for (int g = t >> sh; g < ng; g += TPB >> sh) {
+            const double2 *src = p.part + (int64_t)img * p.S * U + (first + g) * p.P;
+            double a = 0, b = 0;
+#pragma unroll 4
+            for (int e = li; e < n; e += lanes) {
+                const int c = p.P == 1 ? e : e / p.P;
+                const double2 v = src[(int64_t)c * U + (e - c * p.P)];
+                a += v.x, b += v.y;
+            }
+            for (int o = lanes >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o), b += __shfl_xor(b, o);
+            if (li == 0) joined[g] = moments(a, b, (double)p.R * p.cg, p.eps);
+        }
+        __syncthreads();
+    }
     if (!l.live) return;
     const int64_t r0 = chunk * chunk2;
     const int rows = (int)(min(r0 + chunk2, p.R) - r0);
@@ -343,11 +366,18 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int
     uint8_t *oq = TO8 ? p.q + at * p.ldq + s0 : nullptr, *os = TO8 ? p.qs + at * p.ldqs + s0 / kFp8Block : nullptr;
     const int64_t sx = (int64_t)rp * p.ldx;
     Affine<V> f;
+    int g = JOIN ? divided_any(s0 + l.lo, p.cg) : 0, in_g = JOIN ? s0 + l.lo - g * p.cg : 0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int c = s0 + min(l.lo + j, sc - 1);
-        const float2 st = p.stat[(int64_t)img * p.C + c];
-        f.mean[j] = st.x, f.a[j] = st.y;
+        if constexpr (JOIN) {
+            const float2 st = joined[min(g - first, kSliceMax - 1)];
+            f.mean[j] = st.x, f.a[j] = p.w ? st.y * p.w[c] : st.y;
+            if (++in_g == p.cg) in_g = 0, ++g;
+        } else {
+            const float2 st = p.stat[(int64_t)img * p.C + c];
+            f.mean[j] = st.x, f.a[j] = st.y;
+        }
         f.b[j] = p.b ? p.b[c] : 0.f;
     }
     auto emit = [&](const Pack<T, V> &d, int64_t k) {
@@ -564,7 +594,9 @@ template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, 
     if (q.V == 1) norm_stats_kernel<T, 1, true><<<g1, 256, 0, s>>>(n);
     else if (q.one) norm_stats_kernel<T, V, true><<<g1, 256, 0, s>>>(n);
     else norm_stats_kernel<T, V, false><<<g1, 256, 0, s>>>(n);
-    norm_merge_kernel<<<(unsigned)(images * p.G), 256, 0, s>>>(p);
+    // joining costs every workgroup of the last pass what it reads; a launch costs 3 us of the device's time and as much of the host's
+    const bool join = (int64_t)q.S * q.P * p.G <= 1024;
+    if (!join) norm_merge_kernel<<<(unsigned)(images * p.G), 256, 0, s>>>(p);
     // the normalising pass: slices of columns that need not hold whole groups
     const int tail = p.C % kSliceMax, V2 = to8 ? 8 : tail && tail < V ? 1 : V, width = V2 == 1 ? 256 : kSliceMax;
     const int nsl = (p.C + width - 1) / width, sc = std::min(p.C, width);
@@ -576,9 +608,10 @@ template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, 
     if (chunk2 < 4 * rp) chunk2 = 4 * rp;
     S2 = (p.R + chunk2 - 1) / chunk2;
     const unsigned g2 = (unsigned)((int64_t)images * S2 * nsl);
-    if (to8) norm_apply_kernel<T, 8, true><<<g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2);
-    else if (V2 == 1) norm_apply_kernel<T, 1, false><<<g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2);
-    else norm_apply_kernel<T, V, false><<<g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2);
+    auto apply = [&](auto kernel) { kernel<<<g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2); };
+    if (to8) join ? apply(norm_apply_kernel<T, 8, true, true>) : apply(norm_apply_kernel<T, 8, true, false>);
+    else if (V2 == 1) join ? apply(norm_apply_kernel<T, 1, false, true>) : apply(norm_apply_kernel<T, 1, false, false>);
+    else join ? apply(norm_apply_kernel<T, V, false, true>) : apply(norm_apply_kernel<T, V, false, false>);
     return launch_status("group_norm");
 }
 
