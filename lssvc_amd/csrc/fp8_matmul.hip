@@ -240,9 +240,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
     constexpr int NWAVE = (BM / WM) * (BN / WN), FM = WM / 16, FN = WN / 16, STAGE = (BM + BN) * kFp8Block;
     constexpr int PA = BM / 8 / NWAVE, PW = BN / 8 / NWAVE;    // DMA instructions of a wave per block
     constexpr int SLOTS = 2, PD = 1, LAST = FM - PD;
-    constexpr int DPG = (PA + PW) / 4;                         // DMA instructions per fragment of A
+    constexpr int DPG = (PA + PW + 3) / 4;                     // DMA instructions per fragment of A
     constexpr bool WIDE = sizeof(T) == 4;
-    static_assert(WN % 64 == 0 && BM % (8 * NWAVE) == 0 && BN % (8 * NWAVE) == 0 && 128 % WN == 0 && FM % SLOTS == 0 && FM >= 4 && (PA + PW) % 4 == 0, "tile");
+    static_assert(WN % 64 == 0 && BM % (8 * NWAVE) == 0 && BN % (8 * NWAVE) == 0 && 128 % WN == 0 && FM % SLOTS == 0 && FM >= 4, "tile");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, q = lane >> 4;
     // workgroups go to the eight XCDs in turn: give each XCD a run of tiles, walked in bands of 8 tile rows, so that its L2 sees the
@@ -408,14 +408,15 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
 
     if constexpr (BY_PART) add_scaled(acc[FN - 1][FM - 1], late, late_scale);
 
-    // Out through the LDS, 64 x 64 of a wave's tile at a time in a part of its own: whole 128- or 256-byte pieces of rows, and a short loop
+    // Out through the LDS, 64 (or 48) rows of a wave's tile at a time in a part of its own: whole 128- or 256-byte pieces of rows, and a short loop
     // instead of a long unrolled one (a tile's registers cannot be indexed; 16 KB of code cost more to fetch than the tile takes to store).
     // A row's 16-byte chunk c lies at c ^ (row % 16): both directions cover the banks.
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");                    // (fills behind the last block)
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    static_assert(FM % 4 == 0 && FN == 4 && NWAVE * 16384 <= 2 * STAGE, "epilogue");
-    f32x4 *part = (f32x4 *)(lds + wave * 16384);
+    constexpr int HJ = FM % 4 ? 3 : 4;                         // fragments of A at a time
+    static_assert(FM % HJ == 0 && FN == 4 && NWAVE * HJ * 4096 <= 2 * STAGE, "epilogue");
+    f32x4 *part = (f32x4 *)(lds + wave * (HJ * 4096));
     const int c8 = lane & 7, n = n0 + wn + c8 * 8;
     float bias[8];
 #pragma unroll
@@ -426,12 +427,12 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
     const int r0 = lane >> 3, x0 = (c8 * 2) ^ r0, y0 = (c8 * 2 + 1) ^ r0;          // (rows r0 + 8 k: the key alternates between r0 and r0 ^ 8)
     auto out = [&](auto full_, int mh) {
         constexpr bool FULL = decltype(full_)::value;
-        const int rows_left = min(64, p.M - mh);
+        const int rows_left = min(HJ * 16, p.M - mh);
         T *dst = (T *)p.y + (int64_t)(mh + r0) * p.ldy + n;
         const T *res = (const T *)p.res + (p.res ? (int64_t)(mh + r0) * p.ldres + n : 0);
         const f32x4 *from = part + r0 * 16;
 #pragma unroll 2
-        for (int k = 0; k < 8; ++k) {
+        for (int k = 0; k < HJ * 2; ++k) {
             const f32x4 x = from[x0 ^ ((k & 1) * 8)], y = from[y0 ^ ((k & 1) * 8)];
             float v[8] = {x[0] + bias[0], x[1] + bias[1], x[2] + bias[2], x[3] + bias[3], y[0] + bias[4], y[1] + bias[5], y[2] + bias[6], y[3] + bias[7]};
             if (r0 + 8 * k < rows_left && (FULL || n < p.N)) store_cols<FULL, T, 8>(p.act, dst, p.res ? res : nullptr, p.N - n, v);
@@ -441,14 +442,14 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
         }
     };
 #pragma unroll
-    for (int h = 0; h < FM / 4; ++h) {
+    for (int h = 0; h < FM / HJ; ++h) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < HJ; ++j)
 #pragma unroll
-            for (int f = 0; f < 4; ++f) part[(j * 16 + i16) * 16 + ((q * 4 + f) ^ i16)] = acc[f][h * 4 + j];
+            for (int f = 0; f < 4; ++f) part[(j * 16 + i16) * 16 + ((q * 4 + f) ^ i16)] = acc[f][h * HJ + j];
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        if (n0 + BN <= p.N) out(std::true_type{}, m0 + wm + h * 64);
-        else out(std::false_type{}, m0 + wm + h * 64);
+        if (n0 + BN <= p.N) out(std::true_type{}, m0 + wm + h * (HJ * 16));
+        else out(std::false_type{}, m0 + wm + h * (HJ * 16));
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
@@ -492,14 +493,15 @@ template <bool E8M0, typename T> static int launch_matmul(const MatmulP &p, hipS
         const double t = tiles(16 * mf, 16 * nf);
         return 3.0 + t * p.nkb * (mf + nf) * 2048 / (6.5e6 * std::min(1.0, t / 256)) + t / 1024;
     };
-    auto tiled = [&](int bm, double start, double block, double end) { return start + std::ceil(tiles(bm, bm) / 256) * (p.nkb * block + end); };
+    auto tiled = [&](int bm, int bn, double start, double block, double end) { return start + std::ceil(tiles(bm, bn) / 256) * (p.nkb * block + end); };
     // (a pitch that is no multiple of 128: a block of K straddles two lines)
     const double rate = (WIDE ? 1.9 : E8M0 ? 1.0 : 1.17) * ((p.lda | p.ldw) % 128 && p.nkb > 1 ? 1.6 : 1.0);
-    const double cost[6] = {direct(1, 1), direct(1, 4), direct(2, 4), direct(4, 4), tiled(128, 4.5, 0.56 * rate, 1.0), WIDE ? 1e30 : tiled(256, 7.0, 1.42 * rate, 5.0)};
+    const double cost[7] = {direct(1, 1), direct(1, 4), direct(2, 4), direct(4, 4), tiled(128, 128, 4.5, 0.56 * rate, 1.0),
+                            WIDE ? 1e30 : tiled(256, 256, 7.0, 1.42 * rate, 5.0), WIDE ? 1e30 : tiled(192, 256, 6.5, 1.12 * rate, 4.0)};
 #ifdef FP8_SWEEP
-    const int best = getenv("FP8_FORCE") && atoi(getenv("FP8_FORCE")) >= 0 ? atoi(getenv("FP8_FORCE")) : (int)(std::min_element(cost, cost + 6) - cost);
+    const int best = getenv("FP8_FORCE") && atoi(getenv("FP8_FORCE")) >= 0 ? atoi(getenv("FP8_FORCE")) : (int)(std::min_element(cost, cost + 7) - cost);
 #else
-    const int best = (int)(std::min_element(cost, cost + 6) - cost);
+    const int best = (int)(std::min_element(cost, cost + 7) - cost);
 #endif
     switch (best) {
         case 0: return launch_direct<1, 1, E8M0, T>(p, s);
@@ -508,6 +510,9 @@ template <bool E8M0, typename T> static int launch_matmul(const MatmulP &p, hipS
         case 3: return launch_direct<4, 4, E8M0, T>(p, s);
         case 5:
             if constexpr (!WIDE) return launch_tile<256, 256, 128, 64, E8M0, T>(p, s);
+            break;
+        case 6:
+            if constexpr (!WIDE) return launch_tile<192, 256, 96, 64, E8M0, T>(p, s);
             break;
     }
     return launch_tile<128, 128, 64, 64, E8M0, T>(p, s);
