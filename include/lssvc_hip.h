@@ -479,7 +479,8 @@ int lssvc_engine_decode_pframe(void *engine, const uint8_t *bl_file, int64_t bl_
 /* ---- row operators: typed, batched rows ------------------------------------------------------------------------------------
  * A row matrix is what a channels-last map of any batch is: rows = images x H x W, cols = C, `ld` elements between rows. These
  * operators have no counterpart in the reference; they serve transform blocks that normalise over channel groups and take their
- * pointwise products in 8 bits. They are not part of compiled frame plans. */
+ * pointwise products in 8 bits. They are not part of compiled frame plans. What a call writes shares no byte with what it reads, but for
+ * the "may be itself" below; a call that would is refused. */
 enum { LSSVC_F32 = 0, LSSVC_F16 = 1, LSSVC_BF16 = 2 };
 #define LSSVC_ACT_SILU 3 /* x / (1 + exp(-x)); row operators only, beside LSSVC_ACT_* */
 
@@ -509,7 +510,7 @@ typedef struct lssvc_fp8 {
 } lssvc_fp8;
 
 /* Group norm over channel groups, with an activation: per image and group of cols / groups channels
- *   y = act((x - mean) / sqrt(mean((x - mean)^2) + eps) * weight[c] + bias[c]),   statistics in fp32, two-level and shifted.
+ *   y = act((x - mean) / sqrt(mean((x - mean)^2) + eps) * weight[c] + bias[c]),   statistics in fp32 per thread, joined in 64 bits.
  * x holds images x (rows / images) rows. weight / bias: cols fp32 values or NULL (1 / 0). Exactly one of y (x's shape and type;
  * may be x itself) and y8 (1 x 128 blocks, e8m0 scales; the block's scale and values are those lssvc_quantize_fp8 makes of the
  * fp32 result) is given. rows = 0 is no work. workspace: lssvc_group_norm_workspace_bytes(...) bytes, 16-byte aligned, private to
@@ -525,11 +526,11 @@ int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t groups, const 
 int lssvc_quantize_fp8(const lssvc_rows *x, const lssvc_fp8 *y, void *stream);
 
 /* y[m][n] = act(sum_k a[m][k] w[n][k] + bias[n]) + residual[m][n], sums in fp32. a: block_rows 1; w: block_rows 128; both with e8m0
- * scales (applied by the matrix instruction) or both with fp32 scales (applied to each 128-block's partial sum). bias: w->rows fp32
- * values or NULL. residual: y's shape and type or NULL; may be y itself. a->rows = 0 is no work. workspace: as above. */
-int64_t lssvc_matmul_fp8_workspace_bytes(int64_t m, int64_t n, int32_t k);
+ * scales (applied by the matrix instruction) or both with fp32 scales (applied to each 128-block's partial sum; for fp32 results e8m0 scales
+ * are, too). A block's two scales are multiplied with each other in fp32 where they are not the instruction's. bias: w->rows fp32
+ * values or NULL. residual: y's shape and type or NULL; may be y itself. a->rows = 0 is no work. */
 int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const float *bias, int32_t act, float slope, const lssvc_rows *residual,
-                     const lssvc_rows *y, void *workspace, int64_t workspace_bytes, void *stream);
+                     const lssvc_rows *y, void *stream);
 
 /* Runtime tuning switches (each also reads an environment variable at first use):
  *   "f16x3_persist"            1/0   use the persistent warp-specialised 3x3 kernel (LSSVC_F16X3_PERSIST)

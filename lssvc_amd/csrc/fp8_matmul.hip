@@ -31,6 +31,7 @@ struct MatmulP {
     int dtype;
     Act act;
     int tiles_m, tiles_n;
+    int depth;               // LDS stages of a wave (split form)
 };
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -121,82 +122,152 @@ template <int CNT> __device__ __forceinline__ void load_bias(const MatmulP &p, i
     for (int i = 0; i < CNT; ++i) b[i] = p.bias && n + i < p.N ? p.bias[n + i] : 0.f;
 }
 
-template <bool E8M0> __device__ __forceinline__ uint32_t load_scale(const void *s, int64_t at) {
-    if constexpr (E8M0) return ((const uint8_t *)s)[at];
-    else return ((const uint32_t *)s)[at];
+// ---- operands on their way to the LDS ---------------------------------------------------------------------------------------------------
+// Both kernels fill the LDS by DMA, 8 rows x 128 bytes an instruction: whole lines. (Fragments loaded straight into registers are 16 rows x 64
+// bytes an instruction, and the address unit takes 3.5 cycles a line however much of it is used: half the rate, measured.) A row's eight
+// 16-byte chunks are stored permuted, chunk c at c ^ key(row), so that the 16 rows of a fragment read cover all 64 banks; the permutation is
+// applied to the DMA's SOURCE address, its destination is linear.
+__device__ __forceinline__ int key_a(int row) { return (row >> 1) & 7; }                                     // fragment rows: consecutive
+__device__ __forceinline__ int key_w(int row) { return ((row >> 1) & 1) | (((row >> 4) & 3) << 1); }         // fragment rows: 16 (r / 4) + 4 f + r % 4
+
+// a raw buffer of the bytes [p, p + range)
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const uint8_t *p, int range) {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, range, 0x00027000);
+}
+// a value that all lanes share, in scalar registers
+__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
+    const uint64_t v = (uint64_t)p;
+    return (const uint8_t *)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
+}
+// 16 bytes a lane from base + off (bytes; beyond 2^31: zeros) + k to the LDS at `to`, lane after lane
+__device__ __forceinline__ void dma(const uint8_t *base, uint32_t off, int k, uint8_t *to) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(descriptor(base, 0x7fffffff), (__attribute__((address_space(3))) void *)to, 16, off, k, 0, 0);
+}
+constexpr uint32_t kOutside = 0x80000000u;
+// Workgroups go to the eight XCDs in turn: the work of workgroup `id` of `total` if each XCD is to have a run of neighbours
+__device__ __forceinline__ int xcd_run(int id, int total) {
+    const int xcd = id & 7, per = total >> 3, more = total & 7;
+    return xcd * per + min(xcd, more) + (id >> 3);
 }
 
 // ---- small products: bound by the weight's bytes, or by latency ------------------------------------------------------------------------
-// A workgroup owns MF * 16 rows and NF * 16 columns of y; its waves deal K's blocks among themselves, read both operands straight into
-// registers (nothing is read twice within the workgroup, no barrier until the end, little code) and add up through the LDS in a fixed order.
-template <int MF, int NF, bool E8M0, typename T, int NW>
-__global__ __launch_bounds__(NW * 64) void matmul_direct_kernel(MatmulP p) {
-    constexpr int U = MF + NF <= 3 ? 4 : MF + NF <= 5 ? 2 : 1;     // blocks of K in flight per wave
+// A workgroup owns MF * 16 rows and NF * 16 columns of y. Its waves deal K's blocks among themselves: nothing is read twice within the
+// workgroup, each wave fills and reads a part of the LDS of its own, one block ahead, and there is no barrier until the sums are
+// added up through the LDS in a fixed order.
+template <int MF, int NF> struct Split {
+    static constexpr int SCALES = MF == 4 ? 2 : 1;                                  // DMA instructions for a block's scales
+    static constexpr int STAGE = (MF + NF) * 2048 + SCALES * 256, PER = (MF + NF) * 2 + SCALES;     // a block: bytes, DMA instructions
+    static constexpr int WAVES = MF + NF == 2 ? 8 : 4;                              // at most
+    static constexpr int BYTES = WAVES * 2 * STAGE;                                 // LDS, at most
+    static_assert(BYTES <= 160 * 1024 && PER < 64, "split");
+    // blocks for every wave: the same number, but for the last; 16 x 16 tiles are so little work that a wave takes two at least
+    // (24x5000x1000 3.9 us, with one block each 4.4). No more LDS than there are blocks, so that more workgroups share a CU.
+    static int rounds(int nkb) { return std::max((nkb + WAVES - 1) / WAVES, MF + NF == 2 ? std::min(2, nkb) : 1); }
+    static int waves(int nkb) { return (nkb + rounds(nkb) - 1) / rounds(nkb); }
+    static int depth(int nkb) { return rounds(nkb) > 1 ? 2 : 1; }
+    static size_t bytes(int nkb) { return (size_t)waves(nkb) * std::max(depth(nkb) * STAGE, MF * NF * 1024); }
+};
+template <int MF, int NF, bool E8M0, typename T>
+__global__ __launch_bounds__((Split<MF, NF>::WAVES * 64)) void matmul_split_kernel(MatmulP p) {
     constexpr int C = 4 * NF;                                      // consecutive columns of y per lane
     constexpr bool WIDE = sizeof(T) == 4;
+    constexpr int SB = E8M0 ? 1 : 4, SD = Split<MF, NF>::SCALES, STAGE = Split<MF, NF>::STAGE, PER = Split<MF, NF>::PER;
+    const int NW = blockDim.x >> 6, D = p.depth;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
-    f32x4 *red = (f32x4 *)lds;                                     // [wave][column fragment][row fragment][lane]
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i16 = lane & 15, q = lane >> 4;
-    const int tm = blockIdx.x / (unsigned)p.tiles_n, tn = blockIdx.x - tm * p.tiles_n;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, q = lane >> 4;
+    // an XCD takes neighbouring columns with all rows, or neighbouring rows with all columns, whichever there are more of: its L2 sees its
+    // part of the longer operand once (with tiles dealt to the XCDs in turn 767x1945x3004 takes 46 us by 16 x 64, so 29)
+    const bool tall = p.M > p.N;
+    const int id = xcd_run(blockIdx.x, p.tiles_m * p.tiles_n), inner = tall ? p.tiles_n : p.tiles_m;
+    const int outer_at = __builtin_amdgcn_readfirstlane(id / inner), inner_at = id - outer_at * inner;
+    const int tm = tall ? outer_at : inner_at, tn = tall ? inner_at : outer_at;
     const int m0 = tm * (16 * MF), n0 = tn * (16 * NF);
-    const uint8_t *wp[NF], *ap[MF];
-    int64_t sar[MF];
+
+    // DMA: instruction i of an operand covers its rows 8 i ... 8 i + 7
+    const uint8_t *abase = uniform(p.a + (int64_t)m0 * p.lda), *wbase = uniform(p.w + (int64_t)n0 * p.ldw);
+    uint32_t aoff[MF * 2], woff[NF * 2];
+    int wchunk[NF * 2];
+    const int achunk = ((lane & 7) ^ key_a(lane >> 3)) * 16, achunk8 = ((lane & 7) ^ key_a(8 + (lane >> 3))) * 16;
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        const int n = n0 + (NF == 1 ? i16 : (i16 >> 2) * C + f * 4 + (i16 & 3));
-        wp[f] = p.w + (int64_t)min(n, p.N - 1) * p.ldw + q * 16;
-    }
+    for (int i = 0; i < MF * 2; ++i) aoff[i] = (uint32_t)min(i * 8 + (lane >> 3), p.M - 1 - m0) * (uint32_t)p.lda + (i & 1 ? achunk8 : achunk);
 #pragma unroll
-    for (int j = 0; j < MF; ++j) {
-        const int64_t m = min(m0 + j * 16 + i16, p.M - 1);
-        ap[j] = p.a + m * p.lda + q * 16;
-        sar[j] = m * p.ldsa;
+    for (int i = 0; i < NF * 2; ++i) {
+        const int row = i * 8 + (lane >> 3);
+        wchunk[i] = ((lane & 7) ^ (NF == 1 ? key_a(row) : key_w(row))) * 16;
+        woff[i] = (uint32_t)min(row, p.N - 1 - n0) * (uint32_t)p.ldw + wchunk[i];
     }
-    const int64_t swr = (int64_t)(n0 / kFp8Block) * p.ldsw;
+    // scales: lane r takes A's of row r, the lane behind them (of an instruction of its own where there is none) W's
+    const uint8_t *sap = (const uint8_t *)p.sa + (int64_t)min(m0 + min(lane, MF * 16 - 1), p.M - 1) * p.ldsa * SB;
+    const uint8_t *swp = (const uint8_t *)p.sw + (int64_t)(n0 / kFp8Block) * p.ldsw * SB;
+    const uint8_t *first = SD == 1 && lane == MF * 16 ? swp : sap;
+    uint8_t *mine = lds + wave * (D * STAGE);
+    auto fill = [&](int kb, int stage) {
+        uint8_t *to = mine + stage * STAGE;
+        const int k = kb * kFp8Block, at = E8M0 ? kb & ~3 : kb * 4;
+#pragma unroll
+        for (int i = 0; i < MF * 2; ++i) dma(abase, k + (i & 1 ? achunk8 : achunk) < p.K16 ? aoff[i] : kOutside, k, to + i * 1024);
+#pragma unroll
+        for (int i = 0; i < NF * 2; ++i) dma(wbase, k + wchunk[i] < p.K16 ? woff[i] : kOutside, k, to + (MF * 2 + i) * 1024);
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(first + at), (__attribute__((address_space(3))) void *)(to + (MF + NF) * 2048), 4, 0, 0);
+        if constexpr (SD == 2)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(swp + at), (__attribute__((address_space(3))) void *)(to + (MF + NF) * 2048 + 256), 4, 0, 0);
+    };
+
     f32x4 acc[NF][MF] = {};
-    for (int b0 = wave; b0 < p.nkb; b0 += NW * U) {
-        Raw wv[U][NF], av[U][MF];
-        uint32_t ws[U], as[U][MF];
+    const int blocks = wave < p.nkb ? (p.nkb - wave + NW - 1) / NW : 0;
+    for (int d = 0; d < min(D, blocks); ++d) fill(wave + d * NW, d);        // (one block if D = 1)
+    const int wrow = NF == 1 ? i16 : (i16 >> 2) * 16 + (i16 & 3), wkey = NF == 1 ? key_a(wrow) : key_w(wrow);
+    for (int t = 0, stage = 0; t < blocks; ++t) {
+        if (D > 1 && t + 1 < blocks) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PER) : "memory");        // (the next block may be under way)
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const int kb = wave + t * NW;
+        const uint8_t *st = mine + stage * STAGE, *sc = st + (MF + NF) * 2048 + (E8M0 ? kb & 3 : 0);
+        auto scale = [&](int row) {
+            if constexpr (E8M0) return (uint32_t)sc[row * 4];
+            else return *(const uint32_t *)(sc + row * 4);
+        };
+        Raw wv[NF], av[MF];
+        uint32_t as[MF];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int kb = b0 + u * NW, k = kb * kFp8Block;
-            const bool on = kb < p.nkb, lo = on && k + q * 16 < p.K16, hi = on && k + 64 + q * 16 < p.K16;
-            const i32x4 z = {0, 0, 0, 0};
-#pragma unroll
-            for (int f = 0; f < NF; ++f) wv[u][f] = Raw{lo ? *(const i32x4 *)(wp[f] + k) : z, hi ? *(const i32x4 *)(wp[f] + k + 64) : z};
-            ws[u] = on ? load_scale<E8M0>(p.sw, swr + kb) : 0;
-#pragma unroll
-            for (int j = 0; j < MF; ++j) {
-                av[u][j] = Raw{lo ? *(const i32x4 *)(ap[j] + k) : z, hi ? *(const i32x4 *)(ap[j] + k + 64) : z};
-                as[u][j] = on ? load_scale<E8M0>(p.sa, sar[j] + kb) : 0;
-            }
+        for (int f = 0; f < NF; ++f) {
+            const uint8_t *r = st + MF * 2048 + (wrow + f * 4) * kFp8Block;
+            wv[f] = Raw{*(const i32x4 *)(r + ((q ^ wkey) * 16)), *(const i32x4 *)(r + (((q + 4) ^ wkey) * 16))};
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            Frag<WIDE> wf[NF], af;
+        for (int j = 0; j < MF; ++j) {
+            const uint8_t *r = st + (j * 16 + i16) * kFp8Block;
+            av[j] = Raw{*(const i32x4 *)(r + ((q ^ key_a(i16)) * 16)), *(const i32x4 *)(r + (((q + 4) ^ key_a(i16)) * 16))};
+            as[j] = scale(j * 16 + i16);
+        }
+        const uint32_t ws = scale(MF * 16);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // in registers: the stage may be filled again
+        if (t + D < blocks) fill(kb + D * NW, stage);
+        stage = D - 1 - stage;
+        Frag<WIDE> wf[NF], af;
 #pragma unroll
-            for (int f = 0; f < NF; ++f) wf[f].set(wv[u][f].lo, wv[u][f].hi);
+        for (int f = 0; f < NF; ++f) wf[f].set(wv[f].lo, wv[f].hi);
 #pragma unroll
-            for (int j = 0; j < MF; ++j) {
-                af.set(av[u][j].lo, av[u][j].hi);
+        for (int j = 0; j < MF; ++j) {
+            af.set(av[j].lo, av[j].hi);
 #pragma unroll
-                for (int f = 0; f < NF; ++f) mma<E8M0, WIDE>(wf[f], af, acc[f][j], scale_of<E8M0, WIDE>(ws[u]), scale_of<E8M0, WIDE>(as[u][j]));
-            }
+            for (int f = 0; f < NF; ++f) mma<E8M0, WIDE>(wf[f], af, acc[f][j], scale_of<E8M0, WIDE>(ws), scale_of<E8M0, WIDE>(as[j]));
         }
     }
+    __syncthreads();                                               // (every wave's fills have landed and been read)
+    f32x4 *red = (f32x4 *)lds;                                     // [wave][column fragment][row fragment][lane]
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
         for (int j = 0; j < MF; ++j) red[((wave * NF + f) * MF + j) * 64 + lane] = acc[f][j];
     __syncthreads();
-    const int waves = min(NW, p.nkb);                              // (the others had no block)
     for (int e = threadIdx.x; e < MF * 64; e += NW * 64) {
-        const int64_t m = m0 + (e >> 6) * 16 + (e & 15), n = n0 + ((e >> 4) & 3) * C;
+        const int64_t m = m0 + (e >> 6) * 16 + (e & 15);
+        const int n = n0 + ((e >> 4) & 3) * C;
         if (m >= p.M || n >= p.N) continue;
         float v[C];
         load_bias(p, n, v);
         f32x4 s[NF] = {};
-        for (int w = 0; w < waves; ++w)
+        for (int w = 0; w < NW; ++w)
 #pragma unroll
             for (int f = 0; f < NF; ++f) s[f] += red[(w * NF + f) * MF * 64 + e];
 #pragma unroll
@@ -210,31 +281,17 @@ __global__ __launch_bounds__(NW * 64) void matmul_direct_kernel(MatmulP p) {
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------------------
 // BM x BN of y per workgroup, WM x WN per wave. K's blocks pass through two LDS stages of (BM + BN) x 128 bytes, filled by LDS-DMA
-// (16 bytes a lane, no registers). A row's eight 16-byte chunks are stored permuted, chunk c at c ^ key(row), so that the 16 rows of a
-// fragment read cover all 64 banks; the permutation is applied to the DMA's SOURCE address, its destination is linear.
+// (16 bytes a lane, no registers).
 //
 // The matrix units are the bound, so they must not see the LDS: a wave multiplies the fragments of A one after the other against its FN
 // fragments of W and reads PD fragments ahead, over the end of the block too. The one barrier of a block stands PD fragments before its
 // end: there every wave has all of this block in registers and its part of the next one has landed; behind it the stage just read
 // is filled with the block after the next, a quarter of the instructions with each of the next four fragments. (All at once they fill the
 // address unit's queue, and the waves stand in front of it with the matrix units idle: 0.5 us of a block's 1.8 at 256 x 256.)
-__device__ __forceinline__ int key_a(int row) { return (row >> 1) & 7; }                                     // fragment rows: consecutive
-__device__ __forceinline__ int key_w(int row) { return ((row >> 1) & 1) | (((row >> 4) & 3) << 1); }         // fragment rows: 16 (r / 4) + 4 f + r % 4
-
 struct RawA {
     i32x4 lo, hi;
     uint32_t scale;
 };
-// a raw buffer of the bytes [p, p + range)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t descriptor(const uint8_t *p, int range) {
-    return __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, range, 0x00027000);
-}
-// a value that all lanes share, in scalar registers
-__device__ __forceinline__ const uint8_t *uniform(const uint8_t *p) {
-    const uint64_t v = (uint64_t)p;
-    return (const uint8_t *)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
-}
-
 template <int BM, int BN, int WM, int WN, bool E8M0, typename T>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel(MatmulP p) {
     constexpr int NWAVE = (BM / WM) * (BN / WN), FM = WM / 16, FN = WN / 16, STAGE = (BM + BN) * kFp8Block;
@@ -245,14 +302,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
     static_assert(WN % 64 == 0 && BM % (8 * NWAVE) == 0 && BN % (8 * NWAVE) == 0 && 128 % WN == 0 && FM % SLOTS == 0 && FM >= 4, "tile");
     extern __shared__ __attribute__((aligned(16))) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i16 = lane & 15, q = lane >> 4;
-    // workgroups go to the eight XCDs in turn: give each XCD a run of tiles, walked in bands of 8 tile rows, so that its L2 sees the
-    // same operands again
-    const int total = p.tiles_m * p.tiles_n;
-    int id = blockIdx.x;
-    {
-        const int xcd = id & 7, at = id >> 3, per = total >> 3, more = total & 7;
-        id = xcd * per + min(xcd, more) + at;
-    }
+    // an XCD walks its run of tiles in bands of 8 tile rows, so that its L2 sees the same operands again
+    const int id = xcd_run(blockIdx.x, p.tiles_m * p.tiles_n);
     const int band = id / (8 * p.tiles_n), in_band = id - band * 8 * p.tiles_n, rows = min(8, p.tiles_m - band * 8);
     const int tm = __builtin_amdgcn_readfirstlane(band * 8 + in_band % rows), tn = __builtin_amdgcn_readfirstlane(in_band / rows);
     const int m0 = tm * BM, n0 = tn * BN;
@@ -273,16 +324,13 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
         wchunk[i] = ((lane & 7) ^ key_w(drow + i * STEP)) * 16;
         woff[i] = (uint32_t)min(drow + i * STEP, p.N - 1 - n0) * (uint32_t)p.ldw + wchunk[i];
     }
-    auto dma = [&](const uint8_t *base, uint32_t off, int k, int at) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(descriptor(base, 0x7fffffff), (__attribute__((address_space(3))) void *)(lds + at), 16, off, k, 0, 0);
-    };
     auto fill = [&](int kb, int from, int to) {                // DMA instructions from ... to - 1 of a block's
         const int k = min(kb, p.nkb - 1) * kFp8Block, at = (kb & 1) * STAGE + wave * 1024;
 #pragma unroll
         for (int i = 0; i < PA + PW; ++i) {
             if (i < from || i >= to) continue;
-            if (i < PA) dma(abase, k + achunk < p.K16 ? aoff[i] : 0x80000000u, k, at + i * STEP * kFp8Block);
-            else dma(wbase, k + wchunk[i - PA] < p.K16 ? woff[i - PA] : 0x80000000u, k, at + (BM + (i - PA) * STEP) * kFp8Block);
+            if (i < PA) dma(abase, k + achunk < p.K16 ? aoff[i] : kOutside, k, lds + at + i * STEP * kFp8Block);
+            else dma(wbase, k + wchunk[i - PA] < p.K16 ? woff[i - PA] : kOutside, k, lds + at + (BM + (i - PA) * STEP) * kFp8Block);
         }
     };
 
@@ -454,20 +502,17 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
     }
 }
 
-template <int MF, int NF, bool E8M0, typename T, int NW> static int launch_direct(const MatmulP &p, int64_t total, hipStream_t s) {
-    static LdsGrant grant;
-    constexpr size_t bytes = (size_t)NW * MF * NF * 1024;
-    if (int rc = grant.ensure((const void *)matmul_direct_kernel<MF, NF, E8M0, T, NW>, bytes, 64 * 1024)) return rc;
-    matmul_direct_kernel<MF, NF, E8M0, T, NW><<<(unsigned)total, NW * 64, bytes, s>>>(p);
-    return launch_status("matmul_fp8");
-}
-template <int MF, int NF, bool E8M0, typename T> static int launch_direct(MatmulP p, hipStream_t s) {
+template <int MF, int NF, bool E8M0, typename T> static int launch_split(MatmulP p, hipStream_t s) {
+    using Form = Split<MF, NF>;
     p.tiles_m = (p.M + 16 * MF - 1) / (16 * MF);
     p.tiles_n = (p.N + 16 * NF - 1) / (16 * NF);
     const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
-    LSSVC_CHECK(total < (1LL << 31), "matmul_fp8: %lld tiles do not fit one launch", (long long)total);
-    // (8 waves need 8 blocks each has one of; 16 waves are no faster at any size)
-    return p.nkb <= 8 ? launch_direct<MF, NF, E8M0, T, 4>(p, total, s) : launch_direct<MF, NF, E8M0, T, 8>(p, total, s);
+    LSSVC_CHECK(fits_launch(total, Form::waves(p.nkb) * 64), "matmul_fp8: %lld tiles do not fit one launch", (long long)total);
+    p.depth = Form::depth(p.nkb);
+    static LdsGrant grant;
+    if (int rc = grant.ensure((const void *)matmul_split_kernel<MF, NF, E8M0, T>, Form::BYTES, 64 * 1024)) return rc;
+    matmul_split_kernel<MF, NF, E8M0, T><<<(unsigned)total, Form::waves(p.nkb) * 64, Form::bytes(p.nkb), s>>>(p);
+    return launch_status("matmul_fp8");
 }
 
 template <int BM, int BN, int WM, int WN, bool E8M0, typename T> static int launch_tile(MatmulP p, hipStream_t s) {
@@ -477,37 +522,34 @@ template <int BM, int BN, int WM, int WN, bool E8M0, typename T> static int laun
     p.tiles_m = (p.M + BM - 1) / BM;
     p.tiles_n = (p.N + BN - 1) / BN;
     const int64_t total = (int64_t)p.tiles_m * p.tiles_n;
-    LSSVC_CHECK(total < (1LL << 28), "matmul_fp8: %lld tiles do not fit one launch", (long long)total);
+    LSSVC_CHECK(fits_launch(total, (BM / WM) * (BN / WN) * 64), "matmul_fp8: %lld tiles do not fit one launch", (long long)total);
     matmul_tile_kernel<BM, BN, WM, WN, E8M0, T><<<(unsigned)total, (BM / WM) * (BN / WN) * 64, bytes, s>>>(p);
     return launch_status("matmul_fp8");
 }
 
-// Which form: the one with the least estimated time, in us, from times measured at 26 sizes between 1 x 4096 x 4096 and 8192^3 (bf16, e8m0;
-// estimates are within 30 % of them). Direct: 3 us, what its workgroups read (6.5 MB a us if all CUs have one) and 0.25 us for every 256
-// workgroups. Tiles: a start, and for every tile that a CU gets its blocks of K and an end. Two rounds' worth of tiles cost two rounds: the
-// estimate is where the 256 x 256 form's half-empty last round is weighed against the smaller tiles' lower rate.
+// Which form: the one with the least estimated time, in us, fitted to times measured at 72 sizes (1 x 4096 x 4096 ... 8192^3 and random ones,
+// 16-bit and fp32 results, both kinds of scales); the form so chosen takes 1 % more than the fastest one in the geometric mean. Split: a start,
+// and for every tile that a CU gets what it reads and an end; where only one workgroup fits a CU, whole rounds of them. Tiles: the
+// same with whole rounds, since a 256 x 256 form's half-empty last round is what the smaller tiles' lower rate is weighed against.
 template <bool E8M0, typename T> static int launch_matmul(const MatmulP &p, hipStream_t s) {
     constexpr bool WIDE = sizeof(T) == 4;
     auto tiles = [&](int bm, int bn) { return (double)((p.M + bm - 1) / bm) * (double)((p.N + bn - 1) / bn); };
-    auto direct = [&](int mf, int nf) {
-        const double t = tiles(16 * mf, 16 * nf);
-        return 3.0 + t * p.nkb * (mf + nf) * 2048 / (6.5e6 * std::min(1.0, t / 256)) + t / 1024;
+    auto split = [&](auto form, int mf, int nf, double start, double wide, double end) {
+        using Form = decltype(form);
+        const double t = tiles(16 * mf, 16 * nf) / 256, x = 2 * Form::bytes(p.nkb) > 160 * 1024 ? std::ceil(t) : std::max(1.0, t);
+        return start + x * (p.nkb * (mf + nf) * 0.029 * (WIDE ? wide : 1.0) + end);
     };
     auto tiled = [&](int bm, int bn, double start, double block, double end) { return start + std::ceil(tiles(bm, bn) / 256) * (p.nkb * block + end); };
     // (a pitch that is no multiple of 128: a block of K straddles two lines)
-    const double rate = (WIDE ? 1.9 : E8M0 ? 1.0 : 1.17) * ((p.lda | p.ldw) % 128 && p.nkb > 1 ? 1.6 : 1.0);
-    const double cost[7] = {direct(1, 1), direct(1, 4), direct(2, 4), direct(4, 4), tiled(128, 128, 4.5, 0.56 * rate, 1.0),
-                            WIDE ? 1e30 : tiled(256, 256, 7.0, 1.42 * rate, 5.0), WIDE ? 1e30 : tiled(192, 256, 6.5, 1.12 * rate, 4.0)};
-#ifdef FP8_SWEEP
-    const int best = getenv("FP8_FORCE") && atoi(getenv("FP8_FORCE")) >= 0 ? atoi(getenv("FP8_FORCE")) : (int)(std::min_element(cost, cost + 7) - cost);
-#else
-    const int best = (int)(std::min_element(cost, cost + 7) - cost);
-#endif
-    switch (best) {
-        case 0: return launch_direct<1, 1, E8M0, T>(p, s);
-        case 1: return launch_direct<1, 4, E8M0, T>(p, s);
-        case 2: return launch_direct<2, 4, E8M0, T>(p, s);
-        case 3: return launch_direct<4, 4, E8M0, T>(p, s);
+    const double pitch = (p.lda | p.ldw) % 128 && p.nkb > 1 ? 1.6 : 1.0, rate = (E8M0 ? 1.0 : 1.17) * pitch, small_rate = (WIDE ? 2.2 : E8M0 ? 1.0 : 1.2) * pitch;
+    const double cost[7] = {split(Split<1, 1>{}, 1, 1, 2.8, 1.2, 0.08), split(Split<1, 4>{}, 1, 4, 3.1, 1.35, 0.23), split(Split<2, 4>{}, 2, 4, 2.9, 1.55, 0.9),
+                            split(Split<4, 4>{}, 4, 4, 2.0, 1.6, 3.0), tiled(128, 128, 3.8, 0.5 * small_rate, 1.5),
+                            WIDE ? 1e30 : tiled(256, 256, 7.0, 1.38 * rate, 5.0), WIDE ? 1e30 : tiled(192, 256, 6.5, 1.1 * rate, 4.0)};
+    switch (std::min_element(cost, cost + 7) - cost) {
+        case 0: return launch_split<1, 1, E8M0, T>(p, s);
+        case 1: return launch_split<1, 4, E8M0, T>(p, s);
+        case 2: return launch_split<2, 4, E8M0, T>(p, s);
+        case 3: return launch_split<4, 4, E8M0, T>(p, s);
         case 5:
             if constexpr (!WIDE) return launch_tile<256, 256, 128, 64, E8M0, T>(p, s);
             break;
@@ -538,27 +580,23 @@ static int operand_check(const lssvc_fp8 *x, const char *who, int block_rows) {
 
 using namespace lssvc;
 
-extern "C" int64_t lssvc_matmul_fp8_workspace_bytes(int64_t m, int64_t n, int32_t k) {
-    (void)m, (void)n, (void)k;
-    return 0;
-}
-
 extern "C" int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const float *bias, int32_t act, float slope, const lssvc_rows *residual,
-                                const lssvc_rows *y, void *workspace, int64_t workspace_bytes, void *stream) {
-    (void)workspace, (void)workspace_bytes;
+                                const lssvc_rows *y, void *stream) {
     if (int rc = operand_check(a, "a", 1)) return rc;
     if (int rc = operand_check(w, "w", kFp8Block)) return rc;
+    LSSVC_CHECK(w->rows > 0, "matmul_fp8: w has no rows");
     LSSVC_CHECK(a->cols == w->cols, "matmul_fp8: a has %d columns, w has %d", a->cols, w->cols);
     LSSVC_CHECK((a->scale_e8m0 != 0) == (w->scale_e8m0 != 0), "matmul_fp8: one operand has e8m0 scales, the other fp32 scales");
     LSSVC_CHECK(act_ok(act), "matmul_fp8: unknown activation %d", act);
-    LSSVC_CHECK(y && rows_type_ok(y->dtype) && y->rows == a->rows && y->cols == w->rows && y->ld >= y->cols && y->ld < (1LL << 32), "matmul_fp8: the output is not %lld x %lld", (long long)a->rows, (long long)w->rows);
-    if (a->rows == 0 || w->rows == 0) return 0;
-    LSSVC_CHECK(y->ptr && aligned(y->ptr, rows_type_size(y->dtype)), "matmul_fp8: bad output pointer");
+    if (int rc = rows_check("matmul_fp8", y)) return rc;
+    LSSVC_CHECK(y->rows == a->rows && y->cols == w->rows, "matmul_fp8: the output is not %lld x %lld", (long long)a->rows, (long long)w->rows);
     if (residual) {
-        LSSVC_CHECK(residual->ptr && residual->rows == y->rows && residual->cols == y->cols && residual->dtype == y->dtype && residual->ld >= residual->cols && residual->ld < (1LL << 32) &&
-                        aligned(residual->ptr, rows_type_size(y->dtype)), "matmul_fp8: the residual's shape or type is not the output's");
-        LSSVC_CHECK(rows_disjoint_or_same(residual, y), "matmul_fp8: residual and output overlap in part");
+        if (int rc = rows_check("matmul_fp8", residual)) return rc;
+        LSSVC_CHECK(residual->rows == y->rows && residual->cols == y->cols && residual->dtype == y->dtype, "matmul_fp8: the residual's shape or type is not the output's");
     }
+    if (a->rows == 0) return 0;
+    LSSVC_CHECK(!residual || rows_disjoint_or_same(residual, y), "matmul_fp8: residual and output overlap in part");
+    LSSVC_CHECK(apart({span_of(y)}, {values_of(a), scales_of(a), values_of(w), scales_of(w), span_of(bias, w->rows)}), "matmul_fp8: the output overlaps an operand or the bias");
     MatmulP p{};
     p.a = (const uint8_t *)a->values, p.w = (const uint8_t *)w->values;
     p.sa = a->scale, p.sw = w->scale;

@@ -574,7 +574,9 @@ template <typename T, int V, int TPB, bool ONE, bool TO8> static int launch_resi
     n.parts = p.in_place ? 1 : std::max(1, std::min(std::min(8, (its + 1) / 2), 256 / std::min(256, images * q.nslices)));
     n.nv = threads_of<V, TO8>(q.slice), n.m_nv = division_magic(n.nv);
     n.m_uw = division_magic(p.cg), n.m_w = division_magic(ONE ? p.cg / V : p.cg);
-    norm_resident_kernel<T, V, TPB, ONE, TO8><<<(unsigned)(images * q.nslices * n.parts), TPB, q.lds, s>>>(n);
+    const int64_t workgroups = (int64_t)images * q.nslices * n.parts;
+    LSSVC_CHECK(fits_launch(workgroups, TPB), "group_norm: %lld workgroups do not fit one launch", (long long)workgroups);
+    norm_resident_kernel<T, V, TPB, ONE, TO8><<<(unsigned)workgroups, TPB, q.lds, s>>>(n);
     return launch_status("group_norm");
 }
 template <typename T, int TPB> static int launch_resident(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {
@@ -586,29 +588,31 @@ template <typename T, int TPB> static int launch_resident(const NormP &p, const 
 template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {
     if (q.resident) return q.tpb == 256 ? launch_resident<T, 256>(p, q, images, to8, s) : launch_resident<T, 512>(p, q, images, to8, s);
     constexpr int V = kVecOf<T>;
-    const unsigned g1 = (unsigned)((int64_t)images * q.S * q.nslices);
+    const int64_t g1 = (int64_t)images * q.S * q.nslices;
     NormP n = p;
     const int uw = q.P == 1 ? p.cg : q.piece;
     n.nv = q.V == 1 ? q.slice : threads_of<V, false>(q.slice), n.m_nv = division_magic(n.nv);
     n.m_uw = division_magic(uw), n.m_w = division_magic(q.one ? uw / q.V : uw);
-    if (q.V == 1) norm_stats_kernel<T, 1, true><<<g1, 256, 0, s>>>(n);
-    else if (q.one) norm_stats_kernel<T, V, true><<<g1, 256, 0, s>>>(n);
-    else norm_stats_kernel<T, V, false><<<g1, 256, 0, s>>>(n);
-    // joining costs every workgroup of the last pass what it reads; a launch costs 3 us of the device's time and as much of the host's
-    const bool join = (int64_t)q.S * q.P * p.G <= 1024;
-    if (!join) norm_merge_kernel<<<(unsigned)(images * p.G), 256, 0, s>>>(p);
     // the normalising pass: slices of columns that need not hold whole groups
     const int tail = p.C % kSliceMax, V2 = to8 ? 8 : tail && tail < V ? 1 : V, width = V2 == 1 ? 256 : kSliceMax;
     const int nsl = (p.C + width - 1) / width, sc = std::min(p.C, width);
     const int nv = to8 ? threads_of<8, true>(sc) : (sc + V2 - 1) / V2;
     const int64_t rp = 256 / nv;
-    n.nv = nv, n.m_nv = division_magic(nv);
     int64_t S2 = std::max<int64_t>(1, 4096 / std::max<int64_t>(1, (int64_t)images * nsl));
     int64_t chunk2 = (p.R + S2 - 1) / S2;
     if (chunk2 < 4 * rp) chunk2 = 4 * rp;
     S2 = (p.R + chunk2 - 1) / chunk2;
-    const unsigned g2 = (unsigned)((int64_t)images * S2 * nsl);
-    auto apply = [&](auto kernel) { kernel<<<g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2); };
+    const int64_t g2 = images * S2 * nsl;
+    const int64_t g_merge = (int64_t)images * p.G;
+    LSSVC_CHECK(fits_launch(std::max(std::max(g1, g2), g_merge), 256), "group_norm: %d images of %lld rows do not fit one launch", images, (long long)p.R);
+    if (q.V == 1) norm_stats_kernel<T, 1, true><<<(unsigned)g1, 256, 0, s>>>(n);
+    else if (q.one) norm_stats_kernel<T, V, true><<<(unsigned)g1, 256, 0, s>>>(n);
+    else norm_stats_kernel<T, V, false><<<(unsigned)g1, 256, 0, s>>>(n);
+    // joining costs every workgroup of the last pass what it reads; a launch costs 3 us of the device's time and as much of the host's
+    const bool join = (int64_t)q.S * q.P * p.G <= 1024;
+    if (!join) norm_merge_kernel<<<(unsigned)g_merge, 256, 0, s>>>(p);
+    n.nv = nv, n.m_nv = division_magic(nv);
+    auto apply = [&](auto kernel) { kernel<<<(unsigned)g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2); };
     if (to8) join ? apply(norm_apply_kernel<T, 8, true, true>) : apply(norm_apply_kernel<T, 8, true, false>);
     else if (V2 == 1) join ? apply(norm_apply_kernel<T, 1, false, true>) : apply(norm_apply_kernel<T, 1, false, false>);
     else join ? apply(norm_apply_kernel<T, V, false, true>) : apply(norm_apply_kernel<T, V, false, false>);
@@ -624,11 +628,11 @@ int fp8_out_check(const char *what, const lssvc_fp8 *y, int64_t rows, int cols) 
     return 0;
 }
 
-static int rows_check(const char *what, const lssvc_rows *x) {
+int rows_check(const char *what, const lssvc_rows *x) {
     LSSVC_CHECK(x && x->rows >= 0 && (x->ptr || x->rows == 0) && x->cols > 0 && x->ld >= x->cols, "%s: bad rows", what);
     LSSVC_CHECK(rows_type_ok(x->dtype), "%s: unknown element type %d", what, x->dtype);
     LSSVC_CHECK(aligned(x->ptr, rows_type_size(x->dtype)), "%s: rows are not aligned to their element", what);
-    LSSVC_CHECK(x->rows < (1LL << 40) && x->ld < (1LL << 32), "%s: rows %lld x pitch %lld is out of range", what, (long long)x->rows, (long long)x->ld);
+    LSSVC_CHECK(x->rows < (1LL << 40) && x->ld < (1LL << 32) && x->cols <= (1 << 30), "%s: %lld rows x %d, pitch %lld, is out of range", what, (long long)x->rows, x->cols, (long long)x->ld);
     return 0;
 }
 
@@ -650,17 +654,21 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     LSSVC_CHECK(eps >= 0.f, "group_norm: eps %g", eps);
     LSSVC_CHECK(act_ok(act), "group_norm: unknown activation %d", act);
     LSSVC_CHECK((y != nullptr) != (y8 != nullptr), "group_norm: exactly one of the outputs is given");
+    const int64_t R = x->rows / images;
+    const NormPlan q = norm_plan(R, images, x->cols, groups, rows_type_size(x->dtype), y8 != nullptr);
+    const int64_t need = x->rows ? norm_ws(q, images, x->cols, groups) : 0;
+    const Span ws{(uintptr_t)workspace, workspace ? (uint64_t)need : 0};
     if (y) {
         if (int rc = rows_check("group_norm", y)) return rc;
         LSSVC_CHECK(y->rows == x->rows && y->cols == x->cols && y->dtype == x->dtype, "group_norm: the output's shape or type is not the input's");
         if (x->rows) LSSVC_CHECK(rows_disjoint_or_same(x, y), "group_norm: input and output overlap in part");
+        LSSVC_CHECK(apart({span_of(y), ws}, {span_of(weight, x->cols), span_of(bias, x->cols)}), "group_norm: the output overlaps weight, bias or workspace");
     } else if (int rc = fp8_out_check("group_norm", y8, x->rows, x->cols)) return rc;
-    if (y8) LSSVC_CHECK(y8->block_rows == 1, "group_norm: 8-bit output has 1 x 128 blocks");
+    if (y8) {
+        LSSVC_CHECK(y8->block_rows == 1, "group_norm: 8-bit output has 1 x 128 blocks");
+        LSSVC_CHECK(apart({values_of(y8), scales_of(y8), ws}, {span_of(x), span_of(weight, x->cols), span_of(bias, x->cols)}), "group_norm: the output overlaps an input or the workspace");
+    } else LSSVC_CHECK(apart({ws}, {span_of(x)}), "group_norm: the workspace overlaps the input");
     if (x->rows == 0) return 0;
-    const int64_t R = x->rows / images;
-    const int es = rows_type_size(x->dtype);
-    const NormPlan q = norm_plan(R, images, x->cols, groups, es, y8 != nullptr);
-    const int64_t need = norm_ws(q, images, x->cols, groups);
     LSSVC_CHECK(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), "group_norm: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need, (long long)workspace_bytes);
     LSSVC_CHECK(R <= (1LL << 30) && q.P <= kMergeMax, "group_norm: an image of %lld rows x %d channels in %d groups is too large", (long long)R, x->cols, groups);
     LSSVC_CHECK((int64_t)images * std::max<int64_t>(groups, (int64_t)q.nslices * std::max(q.S, 1)) < (1LL << 31), "group_norm: too many images or groups for one launch");

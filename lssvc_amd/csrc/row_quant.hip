@@ -81,29 +81,26 @@ template <typename T> __global__ __launch_bounds__(512) void quant_tiles_kernel(
 template <typename T> static int launch_quant(const QuantP &p, int block_rows, hipStream_t s) {
     if (block_rows == 1) {
         const int64_t blocks = p.rows * p.kb;
-        LSSVC_CHECK((blocks + 15) / 16 < (1LL << 31), "quantize_fp8: %lld blocks do not fit one launch", (long long)blocks);
+        LSSVC_CHECK(fits_launch((blocks + 15) / 16, 256), "quantize_fp8: %lld blocks do not fit one launch", (long long)blocks);
         quant_rows_kernel<T><<<(unsigned)((blocks + 15) / 16), 256, 0, s>>>(p, blocks);
     } else {
         const int64_t tiles = (p.rows + kFp8Block - 1) / kFp8Block * p.kb;
-        LSSVC_CHECK(tiles < (1LL << 31), "quantize_fp8: %lld blocks do not fit one launch", (long long)tiles);
+        LSSVC_CHECK(fits_launch(tiles, 512), "quantize_fp8: %lld blocks do not fit one launch", (long long)tiles);
         quant_tiles_kernel<T><<<(unsigned)tiles, 512, 0, s>>>(p);
     }
     return launch_status("quantize_fp8");
 }
-
-int fp8_out_check(const char *what, const lssvc_fp8 *y, int64_t rows, int cols);
 
 }  // namespace lssvc
 
 using namespace lssvc;
 
 extern "C" int lssvc_quantize_fp8(const lssvc_rows *x, const lssvc_fp8 *y, void *stream) {
-    LSSVC_CHECK(x && x->rows >= 0 && (x->ptr || x->rows == 0) && x->cols > 0 && x->ld >= x->cols && x->rows < (1LL << 40) && x->ld < (1LL << 32), "quantize_fp8: bad rows");
-    LSSVC_CHECK(rows_type_ok(x->dtype), "quantize_fp8: unknown element type %d", x->dtype);
-    LSSVC_CHECK(aligned(x->ptr, rows_type_size(x->dtype)), "quantize_fp8: rows are not aligned to their element");
+    if (int rc = rows_check("quantize_fp8", x)) return rc;
     if (int rc = fp8_out_check("quantize_fp8", y, x->rows, x->cols)) return rc;
     LSSVC_CHECK(y->block_rows == 1 || y->block_rows == kFp8Block, "quantize_fp8: block_rows is 1 or 128, got %d", y->block_rows);
     if (x->rows == 0) return 0;
+    LSSVC_CHECK(apart({values_of(y), scales_of(y)}, {span_of(x)}), "quantize_fp8: input, values and scales overlap");
     QuantP p{x->ptr, (uint8_t *)y->values, (uint8_t *)y->scale, x->ld, y->ld, y->scale_ld, x->rows, x->cols, (x->cols + kFp8Block - 1) / kFp8Block};
     hipStream_t s = (hipStream_t)stream;
     if (x->dtype == LSSVC_F32) return launch_quant<float>(p, y->block_rows, s);

@@ -1,5 +1,6 @@
 // Shared device helpers of the row operators (group norm, block quantiser, 8-bit product): typed rows, activations, 8-bit encoding.
 #pragma once
+#include <initializer_list>
 #include "common.h"
 
 namespace lssvc {
@@ -28,6 +29,39 @@ inline bool rows_disjoint_or_same(const lssvc_rows *a, const lssvc_rows *b) {
     const uint64_t d = pb > pa ? (pb - pa) % la : (la - (pa - pb) % la) % la;       // where b's columns start within a's pitch
     return d >= wa && d + wb <= la;
 }
+
+// A range of bytes that a call reads or writes. What it writes shares no byte with what it reads.
+struct Span {
+    uintptr_t at;
+    uint64_t bytes;
+    bool apart(const Span &o) const { return !bytes || !o.bytes || at + bytes <= o.at || o.at + o.bytes <= at; }
+};
+inline Span span_of(const lssvc_rows *x) {
+    const int es = rows_type_size(x->dtype);
+    return {(uintptr_t)x->ptr, x->rows ? ((uint64_t)(x->rows - 1) * (uint64_t)x->ld + x->cols) * es : 0};
+}
+inline Span span_of(const float *v, int64_t n) { return {(uintptr_t)v, v ? (uint64_t)n * 4 : 0}; }
+inline Span values_of(const lssvc_fp8 *x) {
+    return {(uintptr_t)x->values, x->rows ? (uint64_t)(x->rows - 1) * (uint64_t)x->ld + (x->cols + 15) / 16 * 16 : 0};
+}
+inline Span scales_of(const lssvc_fp8 *x) {
+    const int64_t kb = (x->cols + kFp8Block - 1) / kFp8Block, blocks = x->rows ? (x->rows - 1) / x->block_rows : 0;
+    return {(uintptr_t)x->scale, x->rows ? ((uint64_t)blocks * (uint64_t)x->scale_ld + kb) * (x->scale_e8m0 ? 1 : 4) : 0};
+}
+inline bool apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (const Span *w = written.begin(); w != written.end(); ++w) {
+        for (const Span &r : read)
+            if (!w->apart(r)) return false;
+        for (const Span *o = w + 1; o != written.end(); ++o)
+            if (!w->apart(*o)) return false;
+    }
+    return true;
+}
+// The runtime counts a launch's threads in 32 bits
+inline bool fits_launch(int64_t workgroups, int threads) { return workgroups < (1LL << 31) && workgroups * threads < (1LL << 32); }
+
+int rows_check(const char *what, const lssvc_rows *x);                                       // row_norm.hip
+int fp8_out_check(const char *what, const lssvc_fp8 *y, int64_t rows, int cols);
 
 // ---- typed values: every kernel computes in fp32; storing to 16 bits is the one rounding (to nearest even) ----------------------
 struct bf16_t { uint16_t v; };

@@ -14,6 +14,8 @@ Rows are given as one of
 and come back as the same kind. Everything is enqueued on the current stream of the tensors' device; nothing synchronises. The
 operators are forward operators (a tensor that requires a gradient is refused) and are not part of compiled frame plans.
 """
+import functools
+
 import torch
 
 from . import _lib, hip_ops
@@ -23,6 +25,7 @@ from .hip_ops import T
 BLOCK = 128                                   # columns that share a scale (and rows, in a weight)
 _DTYPE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
 _ACT = {None: _lib.ACT_NONE, "lrelu": _lib.ACT_LRELU, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU}
+_MAX_COLS = 1 << 30
 _E4M3, _E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -45,7 +48,7 @@ def _rows(x, name):
     if not isinstance(x, torch.Tensor):
         _refuse("row_ops: %s is neither a T nor a tensor: %s", name, type(x).__name__)
     dt = _DTYPE.get(x.dtype)
-    if dt is None:
+    if dt is None or x.layout != torch.strided:
         _refuse("row_ops: %s has type %s (fp32, fp16 or bf16 expected)", name, x.dtype)
     if not x.is_cuda:
         _refuse("row_ops: %s is on %s: there is no CPU path", name, x.device)
@@ -55,6 +58,8 @@ def _rows(x, name):
         ld, step = x.stride()
         if (step != 1 and cols > 1) or (ld < cols and rows > 1):
             _refuse("row_ops: the channels of %s are not adjacent (strides %s)", name, tuple(x.stride()))
+        if cols > _MAX_COLS:
+            _refuse("row_ops: %s has %d channels", name, cols)
         return Rows(x.data_ptr(), rows, ld if rows > 1 else cols, cols, dt)
     if x.dim() == 4:
         n, c, h, w = x.shape
@@ -62,6 +67,8 @@ def _rows(x, name):
         ld = sw if w > 1 else sh if h > 1 else sn if n > 1 else c
         if (sc != 1 and c > 1) or ld < c or (h > 1 and sh != w * ld) or (n > 1 and sn != h * w * ld):
             _refuse("row_ops: %s is not channels-last (shape %s, strides %s)", name, tuple(x.shape), tuple(x.stride()))
+        if c > _MAX_COLS:
+            _refuse("row_ops: %s has %d channels", name, c)
         return Rows(x.data_ptr(), n * h * w, ld, c, dt)
     _refuse("row_ops: %s has %d dimensions (rows x channels, or N x C x H x W)", name, x.dim())
 
@@ -116,7 +123,7 @@ class Fp8Rows:
             _refuse("Fp8Rows: block_rows is 1 or %d, got %r", BLOCK, block_rows)
         rows, cols = values.shape
         want = (-(-rows // block_rows), -(-cols // BLOCK))
-        if cols < 1 or tuple(scale.shape) != want:
+        if not 1 <= cols <= _MAX_COLS or tuple(scale.shape) != want:
             _refuse("Fp8Rows: scale is %s, expected %s for %d x %d values in %d x %d blocks", tuple(scale.shape), want, rows, cols, block_rows, BLOCK)
         _no_grad(scale, "scale")
         if rows and not (cols % 16 == 0 and values.stride(1) == 1 and (rows == 1 or values.stride(0) % 16 == 0 and values.stride(0) >= cols) and values.data_ptr() % 16 == 0):
@@ -156,7 +163,7 @@ class Fp8Rows:
         """Uninitialised rows with e8m0 scales, for `out=` of the operators that write 8-bit rows."""
         if block_rows != 1 and block_rows != BLOCK:
             _refuse("Fp8Rows: block_rows is 1 or %d, got %r", BLOCK, block_rows)
-        if rows < 0 or cols < 1:
+        if rows < 0 or not 1 <= cols <= _MAX_COLS:
             _refuse("Fp8Rows: %d x %d values", rows, cols)
         ld, sld = _pitch(cols), -(-cols // (4 * BLOCK)) * 4
         nbytes = rows * ld
@@ -199,6 +206,9 @@ def _fp8_out(out, rows, cols, device, block_rows):
     return out
 
 
+_norm_workspace = functools.lru_cache(1024)(lib.lssvc_group_norm_workspace_bytes)       # (a foreign call takes 1 us)
+
+
 def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
     dev = x.device if isinstance(x, (T, torch.Tensor)) else None
     xr = _rows(x, "x")
@@ -210,6 +220,10 @@ def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
     elif not isinstance(x, T) and x.dim() == 4 and images != x.shape[0]:
         _refuse("group_norm: images=%d, but x has %d", images, x.shape[0])
     rows, cols = xr.rows, xr.cols
+    if rows == 0:
+        images = 1
+    if not 0 < groups <= cols or not 0 < images <= max(rows, 1):
+        _refuse("group_norm: %d rows x %d channels are not %r images, %r groups", rows, cols, images, groups)
     code = _act_code(act)
     wp = None if weight is None else _vector(weight, "weight", cols, dev)
     bp = None if bias is None else _vector(bias, "bias", cols, dev)
@@ -222,18 +236,16 @@ def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
         else:
             _same_device(dev, out=out)
         yr, y8 = _rows(out, "out"), None
-    if rows == 0:
-        images = 1
-    need = lib.lssvc_group_norm_workspace_bytes(rows, images, cols, groups, xr.dtype, fp8)
+    need = _norm_workspace(rows, images, cols, groups, xr.dtype, fp8)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     check(lib.lssvc_group_norm(xr, images, groups, wp, bp, eps, code, slope, yr, y8, ws.data_ptr() if need else None, need, _raw_stream(dev.index)))
     return out
 
 
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None, slope=0.01, images=None, out=None):
-    """act(group_norm(x)): statistics over the rows of each of `images` images and the C / groups channels of a group, in fp32;
-    weight / bias: C fp32 values. images: for 2-d rows and T (default 1); a 4-d tensor brings its own. out: rows of x's shape and type,
-    x itself allowed. act: None, 'lrelu' (slope), 'relu', 'silu'."""
+    """act(group_norm(x)): statistics over the rows of each of `images` images and the C / groups channels of a group, in fp32 per thread,
+    joined in 64 bits; weight / bias: C fp32 values. images: for 2-d rows and T (default 1); a 4-d tensor brings its own. out: rows of
+    x's shape and type, x itself allowed. act: None, 'lrelu' (slope), 'relu', 'silu'."""
     return _group_norm(x, groups, weight, bias, eps, act, slope, images, out, False)
 
 
@@ -288,7 +300,5 @@ def matmul_fp8(a, w, bias=None, *, act=None, slope=0.01, residual=None, out=None
         _refuse("matmul_fp8: dtype %s is not the output's", dtype)
     if w.device != dev or residual is not None and residual.device != dev or out.device != dev:
         _refuse("matmul_fp8: operands on several devices")
-    need = lib.lssvc_matmul_fp8_workspace_bytes(m, n, a.cols)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    check(lib.lssvc_matmul_fp8(a._c, w._c, bp, code, slope, rr, yr, ws.data_ptr() if need else None, need, _raw_stream(dev.index)))
+    check(lib.lssvc_matmul_fp8(a._c, w._c, bp, code, slope, rr, yr, _raw_stream(dev.index)))
     return out

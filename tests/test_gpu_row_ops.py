@@ -240,6 +240,14 @@ MATMUL_CASES = [
     (1, 1, 1), (1, 16, 16), (2, 5, 17), (1, 100, 128), (3, 129, 129), (15, 64, 300), (16, 200, 1000), (17, 77, 515), (31, 300, 2000), (32, 16, 4100),
     (33, 1, 64), (33, 70, 127), (64, 64, 128), (65, 257, 640), (100, 1000, 96), (128, 130, 1030), (200, 200, 200), (257, 511, 384), (400, 1000, 130),
     (1500, 1300, 150), (2100, 2200, 90), (5000, 300, 257), (3300, 4000, 260),
+    # each tiling in its own range (the choice is by estimated time), the last block of K whole and cut, 1 - 4 blocks behind a multiple of 4;
+    # the results' type follows from the sum of the sizes
+    (96, 2644, 3401), (139, 1781, 3991), (146, 1487, 3934), (49, 4027, 4173), (400, 400, 1024),                       # 16 x 64
+    (352, 2870, 3597), (399, 2394, 3862), (341, 2756, 4189), (2330, 430, 4149),                                       # 32 x 64
+    (3850, 253, 4129), (3896, 220, 4174), (4139, 173, 4162), (4866, 81, 1223),                                        # 64 x 64
+    (3942, 4108, 269), (997, 4056, 1149), (3551, 1142, 1102), (4423, 820, 1152),                                      # 128 x 128
+    (3111, 3974, 1037), (4885, 2486, 1043), (3230, 3886, 1028), (4662, 2565, 946),                                    # 256 x 256
+    (3223, 3835, 1019), (3255, 3819, 920), (2841, 4265, 731), (4416, 2712, 464),                                      # 192 x 256
 ]
 
 
@@ -278,6 +286,40 @@ def test_matmul_fp8_epilogues(ops, m, act, dtype):
     bias, res = torch.randn(90, generator=g), torch.randn(m, 90, generator=g).to(dtype)
     want, tol = matmul64(a64, w64, bias, act, res, dtype, slope=0.2)
     within(ops.matmul_fp8(a, w, bias.to(DEV), act=act, slope=0.2, residual=res.to(DEV)), want, tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("m,n", [(40, 70), (700, 600), (3000, 3000)])
+def test_matmul_fp8_operands_at_any_pitch(ops, m, n, dtype):
+    """Slices of wider tensors, read in place: pitches that are no multiple of a line, values behind the last column that are not zero."""
+    g = gen(m + n)
+    for k in (144, 560):
+        wide = lambda rows: (8 * torch.randn(rows, k + 48, generator=g)).to(torch.float8_e4m3fn).to(DEV)[:, 16:16 + k]
+        scales = lambda rows: (0.5 + torch.rand(rows, -(-k // 128) + 3, generator=g)).to(DEV)[:, 1:1 + -(-k // 128)]
+        av, wv, sa, sw = wide(m), wide(n), scales(m), scales(-(-n // 128))
+        a, w = ops.Fp8Rows(av, sa), ops.Fp8Rows(wv, sw, 128)
+        assert a.values.data_ptr() == av.data_ptr() and w.scale.data_ptr() == sw.data_ptr()
+        want, tol = matmul64(dequantize64(av, sa, 1), dequantize64(wv, sw, 128), None, "relu", None, dtype)
+        within(ops.matmul_fp8(a, w, act="relu", dtype=dtype), want, tol)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("m", [20, 1000])
+def test_matmul_fp8_ends_of_the_scales(ops, m, dtype):
+    """The smallest and the largest power of two, whose product is an ordinary one, and the byte that stands for NaN."""
+    g = gen(m)
+    a, w = ops.quantize_fp8(torch.randn(m, 256, generator=g).to(DEV)), ops.quantize_fp8(torch.randn(300, 256, generator=g).to(DEV), 128)
+    sa, sw = torch.full((m, 2), 127, dtype=torch.uint8, device=DEV), torch.full((3, 2), 127, dtype=torch.uint8, device=DEV)
+    sa[:, 0], sw[:, 0] = 0, 254
+    sa[:, 1], sw[:, 1] = 254, 0
+    a, w = ops.Fp8Rows(a.values, sa.view(torch.float8_e8m0fnu)), ops.Fp8Rows(w.values, sw.view(torch.float8_e8m0fnu), 128)
+    want, tol = matmul64(a.values.cpu().double(), w.values.cpu().double(), None, None, None, dtype)
+    within(ops.matmul_fp8(a, w, dtype=dtype), want, tol)
+    sa[:], sw[:] = 127, 127
+    sa[5, 1], sw[1, 0] = 255, 255
+    a, w = ops.Fp8Rows(a.values, sa.view(torch.float8_e8m0fnu)), ops.Fp8Rows(w.values, sw.view(torch.float8_e8m0fnu), 128)
+    want[5], want[:, 128:256] = float("nan"), float("nan")
+    within(ops.matmul_fp8(a, w, dtype=dtype), want, tol)
 
 
 def test_matmul_fp8_blocks_of_very_different_scales(ops):
@@ -399,6 +441,35 @@ def test_the_same_call_twice_gives_the_same_bits(ops):
         assert all(torch.equal(a, b) for a, b in zip(block(ops, s), first))
 
 
+def test_offsets_beyond_32_bits(ops):
+    """More than 2^31 values in and out: the rows at the end are what they are in a call of their own."""
+    g, images, rows, c = gen(7), 270, 65536, 128
+    last = features(g, rows, c, dtype=BF16)
+    x = torch.empty(images * rows, c, dtype=BF16, device=DEV)
+    x.view(images, rows, c)[:] = last.to(DEV)
+    x[:-rows].mul_(-2)
+    y = ops.group_norm(x, 8, act="silu", images=images)
+    want, tol = group_norm64(last, 1, 8, None, None, 1e-5, "silu")
+    within(y[-rows:], want, tol + HALF_STEP[BF16] * (want.abs() + tol) + 2.0 ** -140)
+    del y
+    q = ops.group_norm_fp8(x, 8, act="silu", images=images)
+    own = ops.Fp8Rows(q.values[-rows:], q.scale[-rows:])
+    check_fp8(own, want, tol)
+    del q, own
+    a, tail = ops.quantize_fp8(x), ops.quantize_fp8(x[-500:])
+    assert torch.equal(a.values[-500:].float(), tail.values.float()) and torch.equal(a.scale[-500:].float(), tail.scale.float())
+    w = ops.quantize_fp8(torch.randn(130, c, generator=g).to(DEV), 128)
+    y = ops.matmul_fp8(a, w)
+    want, tol = matmul64(dequantize64(tail.values, tail.scale, 1), dequantize64(w.values, w.scale, 128), None, None, None, BF16)
+    within(y[-500:], want, tol)
+    del y, a
+    v = x.view(128, -1)                                                   # one block of rows, its columns 2^24 values wide
+    w = ops.quantize_fp8(v, 128)
+    want, e = quantize64(v[:, -256:].cpu(), 128)
+    assert torch.equal(w.values[:, -256:].contiguous().cpu().double(), want)
+    assert torch.equal(w.scale[:, -2:].contiguous().view(torch.uint8).cpu().double() - 127, e)
+
+
 def test_no_rows(ops):
     x = torch.empty(0, 48, device=DEV)
     assert ops.group_norm(x, 3).shape == (0, 48)
@@ -442,6 +513,9 @@ def test_refusals_on_the_gpu(ops):
             lambda: ops.matmul_fp8(q, w, residual=torch.zeros(32, 47, device=DEV)), lambda: ops.matmul_fp8(q, w, residual=torch.zeros(32, 48, device=DEV), dtype=F16),
             lambda: ops.matmul_fp8(q, w, out=torch.zeros(31, 48, device=DEV)), lambda: ops.matmul_fp8(q, w, dtype=torch.float64),
             lambda: ops.matmul_fp8(q, w, out=torch.zeros(32, 48, device=DEV), dtype=F16),
+            lambda: ops.group_norm(x, 4 + (1 << 32)), lambda: ops.group_norm(x, 4, images=1 + (1 << 32)),      # not their low 32 bits
+            lambda: ops.group_norm(x, 4, torch.ones(32, 64, device=DEV)[0], out=x[:, :64].t()),
+            lambda: ops.matmul_fp8(q, ops.quantize_fp8(torch.empty(0, 64, device=DEV), 128)),
             lambda: ops.Fp8Rows(q.values, q.scale, 128), lambda: ops.Fp8Rows(q.values, q.scale, 7), lambda: ops.Fp8Rows(x, q.scale),
     ):
         with pytest.raises(E):

@@ -57,8 +57,14 @@ def test_group_norm_refusals():
     refused(norm(y=None, y8=fp8(scale_ld=3)), "multiple of 4")
     refused(norm(y=None, y8=fp8(e8m0=0)), "e8m0")
     refused(norm(y=None, y8=fp8(block_rows=128)), "1 x 128")
+    refused(norm(y=None, y8=fp8(values=4096 + 2032)), "overlaps an input")
+    refused(norm(y=None, y8=fp8(values=1 << 20, scale=4100)), "overlaps an input")
+    refused(norm(x=rows(ld=1 << 32)), "out of range")
     big = rows(rows=1 << 20)
     refused(norm(x=big, y=rows(ptr=1 << 30, rows=1 << 20)), "workspace")
+    refused(norm(x=big, y=rows(ptr=1 << 30, rows=1 << 20), ws=1 << 29, nws=64), "workspace")
+    refused(norm(x=big, y=rows(ptr=1 << 30, rows=1 << 20), ws=(1 << 30) + 4096, nws=1 << 30), "overlaps")
+    refused(norm(x=big, y=rows(ptr=1 << 30, rows=1 << 20), ws=8192, nws=1 << 30), "overlaps")
 
 
 def test_group_norm_workspace_size():
@@ -80,21 +86,32 @@ def test_quantize_refusals():
     refused(q(rows(), fp8(scale=8193)), "4-byte")
     refused(q(rows(), fp8(scale=0)), "no 8-bit output")
     refused(q(rows(), fp8(reserved=1)), "e8m0")
+    refused(q(rows(ptr=4096), fp8()), "overlap")
+    refused(q(rows(ptr=8192 - 2044), fp8(values=1 << 20)), "overlap")                 # the scales, by four bytes
+    refused(q(rows(ptr=1 << 20), fp8(values=8192 - 512 + 16)), "overlap")             # values and scales
+    refused(q(rows(cols=(1 << 30) + 1, ld=1 << 31), fp8()), "out of range")
 
 
 def test_matmul_refusals():
     from lssvc_amd import _lib
     f = lambda a=None, w=None, act=0, res=None, y=None: _lib.lib.lssvc_matmul_fp8(
-        a or fp8(), w or fp8(rows=32, block_rows=128), None, act, 0.01, res, y or rows(ptr=1 << 20, cols=32, ld=32), None, 0, None)
+        a or fp8(), w or fp8(rows=32, block_rows=128), None, act, 0.01, res, y or rows(ptr=1 << 20, cols=32, ld=32), None)
     refused(f(w=fp8(rows=32)), "scales for 1 rows")
     refused(f(a=fp8(block_rows=128)), "scales for 128 rows")
     refused(f(w=fp8(rows=32, cols=63, block_rows=128)), "columns")
     refused(f(w=fp8(rows=32, block_rows=128, e8m0=0)), "e8m0")
+    refused(f(w=fp8(rows=0, block_rows=128)), "no rows")
     refused(f(act=9), "activation")
     refused(f(y=rows(ptr=1 << 20, cols=33, ld=40)), "output")
-    refused(f(y=rows(ptr=1 << 20, cols=32, ld=31)), "output")
-    refused(f(y=rows(ptr=1 << 20, cols=32, ld=32, dtype=5)), "output")
-    refused(f(y=rows(ptr=0, cols=32, ld=32)), "output pointer")
+    refused(f(y=rows(ptr=1 << 20, cols=32, ld=31)), "bad rows")
+    refused(f(y=rows(ptr=1 << 20, cols=32, ld=32, dtype=5)), "type")
+    refused(f(y=rows(ptr=0, cols=32, ld=32)), "bad rows")
+    refused(f(y=rows(ptr=(1 << 20) + 2, cols=32, ld=32)), "aligned")
+    refused(f(y=rows(ptr=4096 + 256, cols=32, ld=32)), "overlaps an operand")         # the values of a and w
+    refused(f(y=rows(ptr=8192, cols=32, ld=32)), "overlaps an operand")               # their scales
+    refused(f(res=rows(ptr=(1 << 22) + 2, cols=32, ld=32)), "aligned")
+    refused(f(a=fp8(rows=1 << 31), y=rows(ptr=1 << 20, rows=1 << 31, cols=32, ld=32)), "too large")
+    refused(f(a=fp8(ld=1 << 22)), "too large")
     refused(f(res=rows(ptr=1 << 22, cols=31, ld=32)), "residual")
     refused(f(res=rows(ptr=1 << 22, cols=32, ld=32, dtype=1)), "residual")
     refused(f(res=rows(ptr=(1 << 20) + 64, cols=32, ld=32)), "overlap")
