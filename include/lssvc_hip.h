@@ -495,8 +495,8 @@ typedef struct lssvc_rows {
 /* 8-bit rows with a scale for each block of block_rows x 128 values: value (r, c) stands for
  * e4m3(values[r * ld + c]) * scale[(r / block_rows) * scale_ld + c / 128] (OCP e4m3: 4 exponent bits, 3 mantissa bits, largest 448).
  * values: 16-byte aligned, ld a multiple of 16; the bytes of columns cols ... next multiple of 16 are zero in every row.
- * Scales: e8m0 (scale_e8m0 = 1: one byte b stands for 2^(b - 127), 255 for NaN; 4-byte aligned, scale_ld a multiple of 4) or
- * fp32 (scale_e8m0 = 0). */
+ * Scales: e8m0 (scale_e8m0 = 1: one byte b stands for 2^(b - 127), 255 for NaN; 4-byte aligned, scale_ld a multiple of 4, every row's
+ * bytes up to the next multiple of 4 can be read) or fp32 (scale_e8m0 = 0). */
 typedef struct lssvc_fp8 {
     void *values;
     void *scale;

@@ -48,21 +48,23 @@ def _rows(x, name):
     if not isinstance(x, torch.Tensor):
         _refuse("row_ops: %s is neither a T nor a tensor: %s", name, type(x).__name__)
     dt = _DTYPE.get(x.dtype)
-    if dt is None or x.layout != torch.strided:
+    if dt is None or x.layout is not torch.strided:
         _refuse("row_ops: %s has type %s (fp32, fp16 or bf16 expected)", name, x.dtype)
     if not x.is_cuda:
         _refuse("row_ops: %s is on %s: there is no CPU path", name, x.device)
-    _no_grad(x, name)
-    if x.dim() == 2:
-        rows, cols = x.shape
+    if x.requires_grad:
+        _no_grad(x, name)
+    shape = x.shape
+    if len(shape) == 2:
+        rows, cols = shape
         ld, step = x.stride()
         if (step != 1 and cols > 1) or (ld < cols and rows > 1):
             _refuse("row_ops: the channels of %s are not adjacent (strides %s)", name, tuple(x.stride()))
         if cols > _MAX_COLS:
             _refuse("row_ops: %s has %d channels", name, cols)
         return Rows(x.data_ptr(), rows, ld if rows > 1 else cols, cols, dt)
-    if x.dim() == 4:
-        n, c, h, w = x.shape
+    if len(shape) == 4:
+        n, c, h, w = shape
         sn, sc, sh, sw = x.stride()
         ld = sw if w > 1 else sh if h > 1 else sn if n > 1 else c
         if (sc != 1 and c > 1) or ld < c or (h > 1 and sh != w * ld) or (n > 1 and sn != h * w * ld):
@@ -74,9 +76,10 @@ def _rows(x, name):
 
 
 def _vector(x, name, n, device):
-    if not (isinstance(x, torch.Tensor) and x.dtype == torch.float32 and x.dim() == 1 and x.shape[0] == n and (n == 1 or x.stride(0) == 1) and x.device == device):
+    if not (isinstance(x, torch.Tensor) and x.dtype is torch.float32 and x.shape == (n,) and x.is_contiguous() and x.is_cuda and x.get_device() == device.index):
         _refuse("row_ops: %s has to be %d adjacent fp32 values on %s", name, n, device)
-    _no_grad(x, name)
+    if x.requires_grad:
+        _no_grad(x, name)
     return x.data_ptr()
 
 
@@ -87,20 +90,16 @@ def _act_code(act):
     return code
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream     # torch.cuda.current_stream(device).cuda_stream without the Stream object (1 us a call)
+# torch.cuda.current_stream(device).cuda_stream without the Stream object, torch.cuda.current_device() without its look at whether the GPU is in
+# use already (a tensor on it says so): 1.3 us of a call's 6 to 8
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _elsewhere(device):
     """Whether `device` has to be made current for a call (every entry point does that around itself)."""
     if hip_ops.PLAN_RECORDER is not None:
         _refuse("row_ops: not part of compiled frame plans")
-    return device.index != torch.cuda.current_device()
-
-
-def _same_device(device, **others):
-    for name, x in others.items():
-        if x is not None and x.device != device:
-            _refuse("row_ops: %s is on %s, the input on %s", name, x.device, device)
+    return device.index != _current_device()
 
 
 class Fp8Rows:
@@ -231,11 +230,16 @@ def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
         out = _fp8_out(out, rows, cols, dev, 1)
         yr, y8 = None, out._c
     else:
-        if out is None:
-            out = T.empty(x.H, x.W, cols, dev) if isinstance(x, T) else torch.empty_like(x)
+        y8 = None
+        if out is None and not isinstance(x, T) and x.dim() == 2:
+            out = torch.empty_like(x) if xr.ld == cols else x.new_empty((rows, cols))
+            yr = Rows(out.data_ptr(), rows, cols, cols, xr.dtype)
         else:
-            _same_device(dev, out=out)
-        yr, y8 = _rows(out, "out"), None
+            if out is None:
+                out = T.empty(x.H, x.W, cols, dev) if isinstance(x, T) else torch.empty_like(x)
+            yr = _rows(out, "out")
+            if out.device != dev:
+                _refuse("row_ops: out is on %s, the input on %s", out.device, dev)
     need = _norm_workspace(rows, images, cols, groups, xr.dtype, fp8)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     check(lib.lssvc_group_norm(xr, images, groups, wp, bp, eps, code, slope, yr, y8, ws.data_ptr() if need else None, need, _raw_stream(dev.index)))

@@ -172,6 +172,24 @@ def test_group_norm_kinds_of_rows(ops):
         ops.group_norm(xd, 5, images=2)
 
 
+@pytest.mark.parametrize("shape", [(2, 20, 1, 10), (2, 20, 6, 1), (3, 20, 1, 1), (1, 20, 1, 1), (2, 1, 4, 5), (0, 20, 3, 3), (2, 20, 0, 3)])
+def test_maps_of_few_pixels_and_slices_of_them(ops, shape):
+    """Shapes whose strides leave open which memory format they are in."""
+    n, c, h, w = shape
+    wide = torch.randn(n, c + 12, h, w, generator=gen(c + h)).to(DEV).to(memory_format=torch.channels_last)
+    x = wide[:, 4:4 + c]
+    rows = x.permute(0, 2, 3, 1).reshape(-1, c)
+    y = ops.group_norm(x, 1, images=None)
+    q = ops.quantize_fp8(x)
+    z = ops.matmul_fp8(q, ops.quantize_fp8(torch.eye(c, device=DEV), 128), residual=x)
+    assert y.shape == x.shape == z.shape and (q.rows, q.cols) == (n * h * w, c)
+    if rows.shape[0]:
+        want, tol = group_norm64(rows.cpu(), n, 1, None, None, 1e-5, None)
+        within(y.permute(0, 2, 3, 1).reshape(-1, c), want, tol + 2.0 ** -24 * want.abs())
+        assert torch.equal(q.values.contiguous().cpu().double(), quantize64(rows.cpu(), 1)[0])
+        assert torch.equal(z.permute(0, 2, 3, 1).reshape(-1, c), q.dequantize() + rows)      # (one product and 0: exact but for the last sum)
+
+
 # ---- quantiser ----------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
 @pytest.mark.parametrize("block_rows", [1, 128])
@@ -374,6 +392,26 @@ def test_norm_product_chain(ops):
     full = f1 @ w2.double().t() + b2 + rows.double()
     err = (y.permute(0, 2, 3, 1).reshape(-1, c).cpu().double() - full).norm() / (full - rows.double()).norm()
     assert err < 2.0 ** -4
+
+
+def test_views_of_the_engine(ops):
+    """hip_ops.T in and out: a slice of a wider buffer as the product's residual and target."""
+    from lssvc_amd.hip_ops import T
+    g = gen(15)
+    x, wide = torch.randn(1, 24, 9, 14, generator=g), torch.randn(1, 40, 9, 14, generator=g)
+    t, s = T.from_nchw(x.to(DEV).contiguous(memory_format=torch.channels_last)), T.from_nchw(wide.to(DEV).contiguous(memory_format=torch.channels_last))
+    part = s.slice(8, 32)
+    q, w = ops.quantize_fp8(t), ops.quantize_fp8(torch.randn(24, 24, generator=g).to(DEV), 128)
+    rows, res = x.permute(0, 2, 3, 1).reshape(-1, 24), wide.permute(0, 2, 3, 1).reshape(-1, 40)
+    assert torch.equal(q.values.contiguous().cpu().double(), quantize64(rows, 1)[0])
+    want, tol = matmul64(dequantize64(q.values, q.scale, 1), dequantize64(w.values, w.scale, 128), None, "relu", res[:, 8:32].contiguous(), F32)
+    y = ops.matmul_fp8(q, w, act="relu", residual=part)
+    assert isinstance(y, T) and (y.H, y.W, y.C) == (9, 14, 24)
+    within(y.to_nchw()[0].permute(1, 2, 0).reshape(-1, 24), want, tol)
+    ops.matmul_fp8(q, w, act="relu", residual=part, out=part)
+    after = s.to_nchw()[0].permute(1, 2, 0).reshape(-1, 40)
+    within(after[:, 8:32], want, tol)
+    assert torch.equal(after[:, :8].cpu(), res[:, :8]) and torch.equal(after[:, 32:].cpu(), res[:, 32:])
 
 
 # ---- calls --------------------------------------------------------------------------------------------------------------------
