@@ -165,7 +165,7 @@ __device__ __forceinline__ void unit_sums(const float (&mean)[V], const float (&
 }
 __device__ __forceinline__ float2 moments(double s1, double s2, double n, float eps) {       // (mean, 1 / sqrt(var + eps))
     const double mean = s1 / n, var = s2 / n - mean * mean;
-    return make_float2((float)mean, 1.f / sqrtf((var < 0 ? 0.f : (float)var) + eps));         // (NaN stays NaN)
+    return make_float2((float)mean, (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + eps)));        // (one rounding each; NaN stays NaN)
 }
 
 // ---- split form, first pass: (S1, S2) of each chunk and unit -----------------------------------------------------------------------
