@@ -153,7 +153,9 @@ __device__ __forceinline__ int xcd_run(int id, int total) {
 // ---- small products: bound by the weight's bytes, or by latency ------------------------------------------------------------------------
 // A workgroup owns MF * 16 rows and NF * 16 columns of y. Its waves deal K's blocks among themselves: nothing is read twice within the
 // workgroup, each wave fills and reads a part of the LDS of its own, one block ahead, and there is no barrier until the sums are
-// added up through the LDS in a fixed order.
+// added up through the LDS in a fixed order. The fewer rows and columns a workgroup has, the more workgroups read W at once: 16 x 16
+// tiles are right for one row (1x4096x4096 4.2 us = 4.0 TB/s from the caches, 5.8 cold; 16 x 64 tiles 6.7), 16 x 64 for 64x4096x4096 (7.4 us; 16 x 16
+// 10.1), 32 x 64 for 128x4096x4096 (8.4; 13.1 by 16 x 64), 64 x 64 for 512x4096x4096 (20; 27 by 32 x 64, 25 by 128 x 128 tiles).
 template <int MF, int NF> struct Split {
     static constexpr int SCALES = MF == 4 ? 2 : 1;                                  // DMA instructions for a block's scales
     static constexpr int STAGE = (MF + NF) * 2048 + SCALES * 256, PER = (MF + NF) * 2 + SCALES;     // a block: bytes, DMA instructions
@@ -288,6 +290,8 @@ __global__ __launch_bounds__((Split<MF, NF>::WAVES * 64)) void matmul_split_kern
 // end: there every wave has all of this block in registers and its part of the next one has landed; behind it the stage just read
 // is filled with the block after the next, a quarter of the instructions with each of the next four fragments. (All at once they fill the
 // address unit's queue, and the waves stand in front of it with the matrix units idle: 0.5 us of a block's 1.8 at 256 x 256.)
+// 8192^3 bf16 by 256 x 256: 400 - 446 us, 2.5 - 2.75 PFLOP/s (library 426 us); a block of K takes 1.03 us on one CU alone and 1.4 with all at work.
+// 4000x2500x4096: 192 x 256 (210 tiles) 46 us, 256 x 256 (160 tiles) 54, 128 x 128 60; with fp32 scales 52, 61, 70.
 struct RawA {
     i32x4 lo, hi;
     uint32_t scale;
