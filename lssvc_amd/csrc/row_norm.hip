@@ -8,7 +8,7 @@
 //   split     rows are split over workgroups that write sums per chunk and group; the chunks are joined by a launch of their own, or, where
 //             they are few, by every workgroup of the normalising pass for itself; that pass reads the map again, in the opposite order,
 //             so that what the first pass read last comes from the caches.
-// Measured: 18x30x64 fp32 4.8 us (resident; a launch that does nothing takes 2.4); 1152x1920x48 fp32 266 us = 113 (3.8 TB/s, what a read-only
+// Measured: 18x30x64 fp32 4.8 us (resident); 1152x1920x48 fp32 266 us = 113 (3.8 TB/s, what a read-only
 // pass reaches) + 5 + 148 (5.7 TB/s); 34560x256 bf16 to 8 bits 7.6 + 3.4 + 10.6 us, of which the activation and the encoding are half.
 // A thread makes (mean, M2) of what it reads, of differences to a value of its own (its share of the squares cannot be lost in them: the
 // value is one of the data), in fp32; from there on sums S1 = sum x and S2 = sum x^2 are in 64 bits, where S2 - S1^2 / N keeps what fp32
