@@ -8,7 +8,7 @@
 //   split     rows are split over workgroups that write sums per chunk and group; the chunks are joined by a launch of their own, or, where
 //             they are few, by every workgroup of the normalising pass for itself; that pass reads the map again, in the opposite order,
 //             so that what the first pass read last comes from the caches.
-// Measured: 18x30x64 fp32 4.8 us (resident); 1152x1920x48 fp32 266 us = 113 (3.8 TB/s, what a read-only
+// Measured: 18x30x64 fp32 4.6 us (resident); 1152x1920x48 fp32 266 us = 113 (3.8 TB/s, what a read-only
 // pass reaches) + 5 + 148 (5.7 TB/s); 34560x256 bf16 to 8 bits 7.6 + 3.4 + 10.6 us, of which the activation and the encoding are half.
 // A thread makes (mean, M2) of what it reads, of differences to a value of its own (its share of the squares cannot be lost in them: the
 // value is one of the data), in fp32; from there on sums S1 = sum x and S2 = sum x^2 are in 64 bits, where S2 - S1^2 / N keeps what fp32
@@ -413,10 +413,11 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int
 // Where there are few groups, several workgroups hold the same slice, make the same statistics of it and share its rows on the way out, which
 // is the longest part (and not possible where x is written over).
 // Rolled loops on purpose: the form serves small maps, whose time is latency, and 50 KB of straight-line code cost more to fetch than the map
-// (27 us for 3 x 1961 x 100 fp16 with the slice in registers and everything unrolled).
+// (27 us for 3 x 1961 x 100 fp16 with the slice in registers and everything unrolled; 8.3 as it is, 8.5 with 4 rows at a time and 10.6 with 8).
+constexpr int kResidentRows = 2; // rows that a thread has under way
 template <typename T, int V, int TPB, bool ONE, bool TO8>
 __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
-    constexpr int NB = 4;
+    constexpr int NB = kResidentRows;
     using D = Pack<T, V>;
     using W = std::conditional_t<(sizeof(D) >= 16), i32x4, T>;  // how a thread's data lies in the LDS
     extern __shared__ __attribute__((aligned(16))) uint8_t dyn[];
@@ -541,7 +542,7 @@ static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8)
     const int64_t nv = to8 ? (slice + kFp8Block - 1) / kFp8Block * (kFp8Block / 8) : (slice + V - 1) / V;
     if (nv <= 512 && R <= kResidentBytes) {
         q.tpb = nv <= 256 && R <= 8 * (256 / nv) ? 256 : 512;
-        const int64_t rp = q.tpb / nv, its = (R + 4 * rp - 1) / (4 * rp) * 4;
+        const int64_t rp = q.tpb / nv, its = (R + kResidentRows * rp - 1) / (kResidentRows * rp) * kResidentRows;
         q.slice = (int)slice;
         q.lds = (size_t)q.tpb * (q.one ? 16 : 8 * V) + (8 * (size_t)(slice / cg) + 15) / 16 * 16 + (size_t)(its * q.tpb * V * es);
         if (q.lds <= kResidentBytes) {
@@ -577,7 +578,7 @@ template <typename T, int V, int TPB, bool ONE, bool TO8> static int launch_resi
     if (int rc = grant.ensure((const void *)norm_resident_kernel<T, V, TPB, ONE, TO8>, q.lds, 64 * 1024)) return rc;
     NormP n = p;
     const int rp = TPB / threads_of<V, TO8>(q.slice), its = (int)((p.R + rp - 1) / rp);
-    n.parts = p.in_place ? 1 : std::max(1, std::min(std::min(8, (its + 1) / 2), 256 / std::min(256, images * q.nslices)));
+    n.parts = p.in_place ? 1 : std::max(1, std::min(std::min(12, its), 256 / std::min(256, images * q.nslices)));
     n.nv = threads_of<V, TO8>(q.slice), n.m_nv = division_magic(n.nv);
     n.m_uw = division_magic(p.cg), n.m_w = division_magic(ONE ? p.cg / V : p.cg);
     const int64_t workgroups = (int64_t)images * q.nslices * n.parts;
