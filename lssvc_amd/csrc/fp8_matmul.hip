@@ -154,8 +154,8 @@ __device__ __forceinline__ int xcd_run(int id, int total) {
 // A workgroup owns MF * 16 rows and NF * 16 columns of y. Its waves deal K's blocks among themselves: nothing is read twice within the
 // workgroup, each wave fills and reads a part of the LDS of its own, one block ahead, and there is no barrier until the sums are
 // added up through the LDS in a fixed order. The fewer rows and columns a workgroup has, the more workgroups read W at once: 16 x 16
-// tiles are right for one row (1x4096x4096 4.2 us = 4.0 TB/s from the caches, 5.8 cold; 16 x 64 tiles 6.7), 16 x 64 for 64x4096x4096 (7.4 us; 16 x 16
-// 10.1), 32 x 64 for 128x4096x4096 (8.4; 13.1 by 16 x 64), 64 x 64 for 512x4096x4096 (20; 27 by 32 x 64, 25 by 128 x 128 tiles).
+// tiles are right for one row (1x4096x4096 4.2 us = 4.0 TB/s from the caches, 5.8 cold; 16 x 64 tiles 6.5), 16 x 64 for 64x4096x4096 (6.9 us; 16 x 16
+// 9.7), 32 x 64 for 128x4096x4096 (8.0; 12.2 by 16 x 64), 64 x 64 for 512x4096x4096 (20; 26 by 32 x 64, 25 by 128 x 128 tiles).
 template <int MF, int NF> struct Split {
     static constexpr int SCALES = MF == 4 ? 2 : 1;                                  // DMA instructions for a block's scales
     static constexpr int STAGE = (MF + NF) * 2048 + SCALES * 256, PER = (MF + NF) * 2 + SCALES;     // a block: bytes, DMA instructions
@@ -171,7 +171,6 @@ template <int MF, int NF> struct Split {
 };
 template <int MF, int NF, bool E8M0, typename T>
 __global__ __launch_bounds__((Split<MF, NF>::WAVES * 64)) void matmul_split_kernel(MatmulP p) {
-    constexpr int C = 4 * NF;                                      // consecutive columns of y per lane
     constexpr bool WIDE = sizeof(T) == 4;
     constexpr int SB = E8M0 ? 1 : 4, SD = Split<MF, NF>::SCALES, STAGE = Split<MF, NF>::STAGE, PER = Split<MF, NF>::PER;
     const int NW = blockDim.x >> 6, D = p.depth;
@@ -215,6 +214,12 @@ __global__ __launch_bounds__((Split<MF, NF>::WAVES * 64)) void matmul_split_kern
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(swp + at), (__attribute__((address_space(3))) void *)(to + (MF + NF) * 2048 + 256), 4, 0, 0);
     };
 
+    // a thread's columns on the way out: a piece of PF fragments; its bias is under way from here
+    constexpr int PF = NF == 4 && !WIDE ? 2 : 1, PIECES = 4 * NF / PF;
+    const int piece = threadIdx.x % PIECES, pq = piece / (NF / PF), pf = piece % (NF / PF) * PF, n = n0 + (pq * NF + pf) * 4;
+    float bias[4 * PF];
+    load_bias(p, n, bias);
+
     f32x4 acc[NF][MF] = {};
     const int blocks = wave < p.nkb ? (p.nkb - wave + NW - 1) / NW : 0;
     for (int d = 0; d < min(D, blocks); ++d) fill(wave + d * NW, d);        // (one block if D = 1)
@@ -256,28 +261,30 @@ __global__ __launch_bounds__((Split<MF, NF>::WAVES * 64)) void matmul_split_kern
         }
     }
     __syncthreads();                                               // (every wave's fills have landed and been read)
-    f32x4 *red = (f32x4 *)lds;                                     // [wave][column fragment][row fragment][lane]
+    // [wave][column fragment][row fragment][lane]; the order of the lanes that share q spreads a row's pieces over the banks
+    f32x4 *red = (f32x4 *)lds;
+    auto at = [&](int f, int j, int fq, int row) { return (f * MF + j) * 64 + ((fq * 16 + row) ^ (((fq + f) & 3) * 4)); };
 #pragma unroll
     for (int f = 0; f < NF; ++f)
 #pragma unroll
-        for (int j = 0; j < MF; ++j) red[((wave * NF + f) * MF + j) * 64 + lane] = acc[f][j];
+        for (int j = 0; j < MF; ++j) red[wave * (NF * MF * 64) + at(f, j, q, i16)] = acc[f][j];
     __syncthreads();
-    for (int e = threadIdx.x; e < MF * 64; e += NW * 64) {
-        const int64_t m = m0 + (e >> 6) * 16 + (e & 15);
-        const int n = n0 + ((e >> 4) & 3) * C;
-        if (m >= p.M || n >= p.N) continue;
-        float v[C];
-        load_bias(p, n, v);
-        f32x4 s[NF] = {};
+    if (n >= p.N) return;
+    // out in 16-byte pieces, neighbouring threads along a row
+#pragma unroll 1
+    for (int row = threadIdx.x / PIECES; row < min(MF * 16, p.M - m0); row += NW * (64 / PIECES)) {
+        float v[4 * PF];
+        f32x4 s[PF] = {};
+#pragma unroll 4
         for (int w = 0; w < NW; ++w)
 #pragma unroll
-            for (int f = 0; f < NF; ++f) s[f] += red[(w * NF + f) * MF * 64 + e];
+            for (int f = 0; f < PF; ++f) s[f] += red[w * (NF * MF * 64) + at(pf + f, row >> 4, pq, row & 15)];
 #pragma unroll
-        for (int c = 0; c < C; ++c) v[c] += s[c >> 2][c & 3];
-        T *dst = (T *)p.y + m * p.ldy + n;
-        const T *res = p.res ? (const T *)p.res + m * p.ldres + n : nullptr;
-        if (n0 + 16 * NF <= p.N) store_cols<true, T, C>(p.act, dst, res, C, v);        // (the workgroup agrees)
-        else store_cols<false, T, C>(p.act, dst, res, p.N - n, v);
+        for (int c = 0; c < 4 * PF; ++c) v[c] = s[c >> 2][c & 3] + bias[c];
+        T *dst = (T *)p.y + (int64_t)(m0 + row) * p.ldy + n;
+        const T *res = p.res ? (const T *)p.res + (int64_t)(m0 + row) * p.ldres + n : nullptr;
+        if (n0 + 16 * NF <= p.N) store_cols<true, T, 4 * PF>(p.act, dst, res, 4 * PF, v);        // (the workgroup agrees)
+        else store_cols<false, T, 4 * PF>(p.act, dst, res, p.N - n, v);
     }
 }
 
@@ -538,17 +545,18 @@ template <int BM, int BN, int WM, int WN, bool E8M0, typename T> static int laun
 template <bool E8M0, typename T> static int launch_matmul(const MatmulP &p, hipStream_t s) {
     constexpr bool WIDE = sizeof(T) == 4;
     auto tiles = [&](int bm, int bn) { return (double)((p.M + bm - 1) / bm) * (double)((p.N + bn - 1) / bn); };
-    auto split = [&](auto form, int mf, int nf, double start, double wide, double end) {
+    auto split = [&](auto form, int mf, int nf, double start, double read, double wide, double end) {
         using Form = decltype(form);
         const double t = tiles(16 * mf, 16 * nf) / 256, x = 2 * Form::bytes(p.nkb) > 160 * 1024 ? std::ceil(t) : std::max(1.0, t);
-        return start + x * (p.nkb * (mf + nf) * 0.029 * (WIDE ? wide : 1.0) + end);
+        return start + x * (p.nkb * (mf + nf) * read * (WIDE ? wide : 1.0) + end);
     };
     auto tiled = [&](int bm, int bn, double start, double block, double end) { return start + std::ceil(tiles(bm, bn) / 256) * (p.nkb * block + end); };
     // (a pitch that is no multiple of 128: a block of K straddles two lines)
     const double pitch = (p.lda | p.ldw) % 128 && p.nkb > 1 ? 1.6 : 1.0, rate = (E8M0 ? 1.0 : 1.17) * pitch, small_rate = (WIDE ? 2.2 : E8M0 ? 1.0 : 1.2) * pitch;
-    const double cost[7] = {split(Split<1, 1>{}, 1, 1, 2.8, 1.2, 0.08), split(Split<1, 4>{}, 1, 4, 3.1, 1.35, 0.23), split(Split<2, 4>{}, 2, 4, 2.9, 1.55, 0.9),
-                            split(Split<4, 4>{}, 4, 4, 2.0, 1.6, 3.0), tiled(128, 128, 3.8, 0.5 * small_rate, 1.5),
-                            WIDE ? 1e30 : tiled(256, 256, 7.0, 1.38 * rate, 5.0), WIDE ? 1e30 : tiled(192, 256, 6.5, 1.1 * rate, 4.0)};
+    const double cost[7] = {split(Split<1, 1>{}, 1, 1, 2.8, 0.028, 1.25, 0.07), split(Split<1, 4>{}, 1, 4, 3.1, 0.028, 1.38, 0.18),
+                            split(Split<2, 4>{}, 2, 4, 2.9, 0.029, 1.55, 0.9), split(Split<4, 4>{}, 4, 4, 2.6, 0.03, 1.65, 2.4),
+                            tiled(128, 128, 4.3, 0.5 * small_rate, 2.5), WIDE ? 1e30 : tiled(256, 256, 7.0, 1.38 * rate, 5.0),
+                            WIDE ? 1e30 : tiled(192, 256, 6.5, 1.1 * rate, 4.0)};
     switch (std::min_element(cost, cost + 7) - cost) {
         case 0: return launch_split<1, 1, E8M0, T>(p, s);
         case 1: return launch_split<1, 4, E8M0, T>(p, s);

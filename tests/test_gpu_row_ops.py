@@ -262,7 +262,7 @@ MATMUL_CASES = [
     # the results' type follows from the sum of the sizes
     (96, 2644, 3401), (139, 1781, 3991), (146, 1487, 3934), (49, 4027, 4173), (400, 400, 1024),                       # 16 x 64
     (352, 2870, 3597), (399, 2394, 3862), (341, 2756, 4189), (2330, 430, 4149),                                       # 32 x 64
-    (3850, 253, 4129), (3896, 220, 4174), (4139, 173, 4162), (4866, 81, 1223),                                        # 64 x 64
+    (3850, 253, 4129), (3896, 220, 4174), (4139, 173, 4162), (3970, 205, 406),                                         # 64 x 64
     (3942, 4108, 269), (997, 4056, 1149), (3551, 1142, 1102), (4423, 820, 1152),                                      # 128 x 128
     (3111, 3974, 1037), (4885, 2486, 1043), (3230, 3886, 1028), (4662, 2565, 946),                                    # 256 x 256
     (3223, 3835, 1019), (3255, 3819, 920), (2841, 4265, 731), (4416, 2712, 464),                                      # 192 x 256
