@@ -539,7 +539,7 @@ template <int BM, int BN, int WM, int WN, bool E8M0, typename T> static int laun
 }
 
 // Which form: the one with the least estimated time, in us, fitted to times measured at 72 sizes (1 x 4096 x 4096 ... 8192^3 and random ones,
-// 16-bit and fp32 results, both kinds of scales); the form so chosen takes 1 % more than the fastest one in the geometric mean. Split: a start,
+// 16-bit and fp32 results, both kinds of scales); the form so chosen takes 0.5 % more than the fastest one in the geometric mean. Split: a start,
 // and for every tile that a CU gets what it reads and an end; where only one workgroup fits a CU, whole rounds of them. Tiles: the
 // same with whole rounds, since a 256 x 256 form's half-empty last round is what the smaller tiles' lower rate is weighed against.
 template <bool E8M0, typename T> static int launch_matmul(const MatmulP &p, hipStream_t s) {
