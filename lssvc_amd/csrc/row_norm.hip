@@ -575,7 +575,8 @@ static int64_t norm_ws(const NormPlan &q, int images, int C, int G) {
 
 template <typename T, int V, int TPB, bool ONE, bool TO8> static int launch_resident(const NormP &p, const NormPlan &q, int images, hipStream_t s) {
     static LdsGrant grant;
-    if (int rc = grant.ensure((const void *)norm_resident_kernel<T, V, TPB, ONE, TO8>, q.lds, 64 * 1024)) return rc;
+    if (q.lds > 64 * 1024)                                       // (all there is, once: two threads' calls never lower each other's limit)
+        if (int rc = grant.ensure((const void *)norm_resident_kernel<T, V, TPB, ONE, TO8>, kResidentBytes, 64 * 1024)) return rc;
     NormP n = p;
     const int rp = TPB / threads_of<V, TO8>(q.slice), its = (int)((p.R + rp - 1) / rp);
     n.parts = p.in_place ? 1 : std::max(1, std::min(std::min(12, its), 256 / std::min(256, images * q.nslices)));

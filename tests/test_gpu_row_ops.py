@@ -48,7 +48,7 @@ NORM_CASES = [
     # groups wider than a slice, as many groups as channels
     (1, 1, 1, 1), (1, 1, 8, 2), (2, 3, 3, 1), (1, 5, 7, 7), (3, 4, 9, 3), (1, 64, 16, 4), (2, 100, 20, 5), (1, 540, 64, 8), (5, 17, 48, 8),
     (1, 1000, 33, 11), (1, 2160, 12, 12), (2, 2160, 96, 3), (1, 333, 1000, 8), (1, 9, 5000, 2), (1, 3, 8200, 2), (1, 700, 4104, 1),
-    (1, 20000, 24, 3), (1, 5000, 1027, 1027), (1, 4000, 2060, 1), (1, 6000, 2049, 3), (1, 3000, 1030, 103), (2, 5000, 100, 5), (1, 9000, 130, 1), (1, 40000, 8, 8), (1, 70000, 3, 1), (130, 40, 64, 4),
+    (1, 20000, 24, 3), (1, 5000, 1027, 1027), (1, 4000, 2060, 1), (1, 6000, 2049, 3), (1, 3000, 1030, 103), (2, 5000, 100, 5), (1, 9000, 130, 1), (1, 40000, 8, 8), (1, 70000, 3, 1), (130, 40, 64, 4), (3000, 1, 40, 4), (700, 2, 6, 2),
 ]
 
 
@@ -148,6 +148,17 @@ def test_group_norm_constant_groups_give_the_bias(ops):
     for rows in (6, 50000):
         y = ops.group_norm(torch.full((rows, 24), 3.25, device=DEV), 3, None, b)
         assert torch.equal(y, b.expand(rows, 24))
+
+
+@pytest.mark.parametrize("rows,c,groups", [(50, 40, 5), (2000, 33, 11), (30000, 96, 4), (20000, 260, 130)])
+def test_group_norm_with_one_of_weight_and_bias(ops, rows, c, groups):
+    g = gen(c)
+    x, v = features(g, rows, c), 0.5 + torch.rand(c, generator=g)
+    for w, b in ((v, None), (None, v)):
+        want, tol = group_norm64(x, 1, groups, w, b, 1e-5, "relu")
+        dw, db = (None if t is None else t.to(DEV) for t in (w, b))
+        within(ops.group_norm(x.to(DEV), groups, dw, db, act="relu"), want, tol + 2.0 ** -24 * want.abs())
+        check_fp8(ops.group_norm_fp8(x.to(DEV), groups, dw, db, act="relu"), want, tol)
 
 
 def test_group_norm_kinds_of_rows(ops):
@@ -258,6 +269,7 @@ MATMUL_CASES = [
     (1, 1, 1), (1, 16, 16), (2, 5, 17), (1, 100, 128), (3, 129, 129), (15, 64, 300), (16, 200, 1000), (17, 77, 515), (31, 300, 2000), (32, 16, 4100),
     (33, 1, 64), (33, 70, 127), (64, 64, 128), (65, 257, 640), (100, 1000, 96), (128, 130, 1030), (200, 200, 200), (257, 511, 384), (400, 1000, 130),
     (1500, 1300, 150), (2100, 2200, 90), (5000, 300, 257), (3300, 4000, 260),
+    (2, 5, 100003), (70, 130, 50000), (1, 200001, 20), (20001, 1, 130),                                               # long, wide, tall
     # each tiling in its own range (the choice is by estimated time), the last block of K whole and cut, 1 - 4 blocks behind a multiple of 4;
     # the results' type follows from the sum of the sizes
     (96, 2644, 3401), (139, 1781, 3991), (146, 1487, 3934), (49, 4027, 4173), (400, 400, 1024),                       # 16 x 64
@@ -470,6 +482,28 @@ def test_calls_on_two_streams_at_once(ops):
     for k in range(2):
         for r in got[k]:
             assert all(torch.equal(o, w) for o, w in zip(r, want[k]))
+
+
+def test_calls_from_two_threads(ops):
+    """Every thread on a stream of its own, maps whose slices take different amounts of LDS."""
+    import threading
+    states = [[torch.randn(rows, 64, generator=gen(rows)).to(DEV) for rows in sizes] for sizes in ((300, 2400), (1200, 1900))]
+    want = [[ops.group_norm(x, 8, act="silu") for x in s] for s in states]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                got = [ops.group_norm(x, 8, act="silu") for x in states[k]]
+            torch.cuda.current_stream().synchronize()
+            wrong.extend(k for a, b in zip(got, want[k]) if not torch.equal(a, b))
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert wrong == []
 
 
 def test_the_same_call_twice_gives_the_same_bits(ops):
