@@ -510,7 +510,7 @@ typedef struct lssvc_fp8 {
 } lssvc_fp8;
 
 /* Group norm over channel groups, with an activation: per image and group of cols / groups channels
- *   y = act((x - mean) / sqrt(mean((x - mean)^2) + eps) * weight[c] + bias[c]),   statistics in fp32 per thread, joined in 64 bits.
+ *   y = act((x - mean) / sqrt(mean((x - mean)^2) + eps) * weight[c] + bias[c]),   sums in 64 bits.
  * x holds images x (rows / images) rows. weight / bias: cols fp32 values or NULL (1 / 0). Exactly one of y (x's shape and type;
  * may be x itself) and y8 (1 x 128 blocks, e8m0 scales; the block's scale and values are those lssvc_quantize_fp8 makes of the
  * fp32 result) is given. rows = 0 is no work. workspace: lssvc_group_norm_workspace_bytes(...) bytes, 16-byte aligned, private to

@@ -10,9 +10,10 @@
 //             so that what the first pass read last comes from the caches.
 // Measured: 18x30x64 fp32 4.6 us (resident); 1152x1920x48 fp32 266 us = 113 (3.8 TB/s, what a read-only
 // pass reaches) + 5 + 148 (5.7 TB/s); 34560x256 bf16 to 8 bits 7.6 + 3.4 + 10.6 us, of which the activation and the encoding are half.
-// A thread makes (mean, M2) of what it reads, of differences to a value of its own (its share of the squares cannot be lost in them: the
-// value is one of the data), in fp32; from there on sums S1 = sum x and S2 = sum x^2 are in 64 bits, where S2 - S1^2 / N keeps what fp32
-// data can hold: an offset a thousand times the spread costs 2^-33 of the variance.
+// Sums S1 = sum x and S2 = sum x^2 are in 64 bits from the first value on: squares of fp32 and bf16 values leave fp32's range (from 1.8e19 and
+// below 1e-19 on), and S2 - S1^2 / N keeps what fp32 data can hold: an offset a thousand times the spread costs 2^-33 of the variance. A value
+// costs a conversion, an addition and an FMA, which run at the rate of fp32 ones. The mean is held as two fp32 numbers, the second folded
+// into the shift, so an offset costs no digits of the result.
 //
 // One thread handles V consecutive channels: 16 bytes at any alignment (8 channels where 8-bit blocks are written). Where V does not divide
 // the slice, a row's last thread loads the LAST V channels -- wide loads only -- and owns those that its neighbour does not (a slice of fewer
@@ -32,7 +33,7 @@ struct NormP {
     int64_t R;                   // rows of an image
     const float *w, *b;
     double2 *part;               // split form: [image][unit][chunk] (S1, S2): whole lines for those who add a unit up
-    float *mean, *scale;         // split form: [image][channel] mean, weight / sqrt(var + eps)
+    float *mean, *scale, *shift; // split form: [image][channel] mean, weight / sqrt(var + eps), bias less the mean's second part
     int64_t chunk;               // rows of a chunk
     int C, G, cg;
     int S;                       // chunks of an image
@@ -68,12 +69,12 @@ template <int V> struct Lane {
     }
     __device__ __forceinline__ bool owns(int j) const { return j >= own && j < end; }
     // the unit (group, or piece) of each channel: units are `uw` wide and start at the slice's first column
-    template <bool ONE> __device__ __forceinline__ void units(int uw, uint32_t m_uw, int nu, int (&un)[V]) const {
+    template <bool ALIKE> __device__ __forceinline__ void units(int uw, uint32_t m_uw, int nu, int (&un)[V]) const {
         int u = divided(lo, m_uw), c = lo - u * uw;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             un[j] = min(u, nu - 1);
-            if (!ONE && ++c == uw) c = 0, ++u;
+            if (!ALIKE && ++c == uw) c = 0, ++u;
         }
     }
 };
@@ -94,87 +95,128 @@ template <typename T, int V, bool NARROW = false> __device__ __forceinline__ Pac
     return r;
 }
 
-// (S1, S2) of every unit of a slice from the threads' (mean, M2) of n rows each: entries go to the LDS, a unit's are added up by 2^sh lanes
-// (of several waves where there are fewer units than waves) in a fixed order, and one lane hands the totals to `done`. ONE: V divides the
-// unit width, a thread's channels lie in one unit and are added before. A thread's n is `q` or, for the first `rem` rows in flight, q + 1.
-template <int TPB, int V, bool ONE> constexpr int kEntryBytes = ONE ? TPB * 16 : TPB * V * 8;
-template <int TPB, int V, bool ONE, typename F>
-__device__ __forceinline__ void unit_sums(const float (&mean)[V], const float (&m2)[V], int q, int rem, const Lane<V> &l, int nv, int rp, int sc, int uw, uint32_t m_w,
-                                          int nu, void *entries, F done) {
+// (S1, S2) of every unit of a slice from the threads' sums: entries go to the LDS, a unit's are added up by 2^sh lanes (of several waves where
+// there are fewer units than waves) in a fixed order, and one lane hands the totals on. What a thread enters:
+//   ONE   V divides the unit width: its V channels lie in one unit, one pair
+//   TWO   they lie in two units at most: a pair for each
+//   EACH  narrow units: a pair for every channel
+//   TURNS the same in half the LDS, for a map that needs the rest: S1 first and S2 after it, unit u's totals by the same lane (2160x12 fp16 in
+//         12 groups 8.6 us, by EACH 7.1; 3x1961x100 fp16 9.5, by TWO 8.0)
+enum Sums { ONE, TWO, EACH, TURNS };
+__host__ __device__ constexpr Sums sums_of(int uw, int V) { return uw % V == 0 ? ONE : uw >= V - 1 || 2 * uw == V ? TWO : EACH; }
+__host__ __device__ constexpr int entries_of(Sums how, int uw, int V) { return how == ONE ? uw / V : how == TWO ? (uw + V - 2) / V + 1 : uw; }   // of a unit in a row, at most
+// 64-bit sums that a thread keeps: one for each channel; where all of them lie in one unit, enough that an addition need not wait for the one before
+template <int V, Sums HOW> constexpr int kChains = HOW == ONE && V > 2 ? 2 : V;
+constexpr int entry_bytes(int threads, Sums how, int V) { return threads * (how == ONE ? 16 : how == TWO ? 32 : how == EACH ? 16 * V : 8 * V); }
+__device__ __forceinline__ double2 operator+(const double2 &a, const double2 &b) { return make_double2(a.x + b.x, a.y + b.y); }
+__device__ __forceinline__ double wave_total(double a) { return wave_sum_hi(a); }
+__device__ __forceinline__ double2 wave_total(const double2 &a) { return make_double2(wave_sum_hi(a.x), wave_sum_hi(a.y)); }
+__device__ __forceinline__ double from_lane(double a, int o) { return __shfl_xor(a, o); }
+__device__ __forceinline__ double2 from_lane(const double2 &a, int o) { return make_double2(__shfl_xor(a.x, o), __shfl_xor(a.y, o)); }
+// `entry(u, r, c)`: the c-th of W of unit u in row r
+template <int TPB, typename E, typename G, typename F> __device__ __forceinline__ void add_up(int W, uint32_t m_w, int rows, int nu, G entry, F done) {
+    __shared__ E wsum[TPB / 64];
     const int t = threadIdx.x;
-    __shared__ double2 wsum[TPB / 64];
-    double2 *one = (double2 *)entries;
-    float2 *each = (float2 *)entries;
-    if (l.live) {
-        if constexpr (ONE) {
-            const double n = q + (l.rt < rem ? 1 : 0);
-            double a = 0, b = 0;
-            float m = 0.f;
-#pragma unroll
-            for (int j = 0; j < V; ++j) a += mean[j], b = fma((double)mean[j], (double)mean[j], b), m += m2[j];
-            one[l.rt * nv + l.cv] = n > 0 ? make_double2(n * a, fma(n, b, (double)m)) : make_double2(0, 0);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (l.owns(j)) each[l.rt * sc + l.lo + j] = make_float2(mean[j], m2[j]);
-        }
-    }
-    __syncthreads();
-    const int W = ONE ? uw / V : uw, pitch = ONE ? nv : sc;
-    const int live_rows = q > 0 ? rp : rem;                    // rows in flight that hold anything
     int sh = TPB == 512 ? 9 : 8;
     while (sh > 0 && (nu << sh) > TPB) --sh;
     const int lpu = 1 << sh, li = t & (lpu - 1);
     const int dr = divided(lpu, m_w), dc = lpu - dr * W;
-    int r = divided(li, m_w), c = li - r * W;
-    const int r0 = r, c0 = c;
+    const int r0 = divided(li, m_w), c0 = li - r0 * W;
     for (int u = t >> sh; u < nu; u += TPB >> sh) {
-        double a = 0, b = 0;
-        r = r0, c = c0;
+        E a{};
+        int r = r0, c = c0;
 #pragma unroll 2
-        while (r < live_rows) {
-            const int at = r * pitch + u * W + c;
-            if constexpr (ONE) a += one[at].x, b += one[at].y;
-            else {
-                const float2 e = each[at];
-                const double n = q + (r < rem ? 1 : 0), m = e.x;
-                a = fma(n, m, a);
-                b += fma(n * m, m, (double)e.y);
-            }
+        while (r < rows) {
+            a = a + entry(u, r, c);
             r += dr;
             c += dc;
             if (c >= W) c -= W, ++r;
         }
         if (sh >= 6) {
-            a = wave_sum_hi(a), b = wave_sum_hi(b);
+            a = wave_total(a);
             if ((t & 63) == 63) {
-                if (sh == 6) done(u, a, b);
-                else wsum[t >> 6] = make_double2(a, b);
+                if (sh == 6) done(u, a);
+                else wsum[t >> 6] = a;
             }
         } else {
-            for (int o = lpu >> 1; o > 0; o >>= 1) a += __shfl_xor(a, o), b += __shfl_xor(b, o);
-            if (li == 0) done(u, a, b);
+            for (int o = lpu >> 1; o > 0; o >>= 1) a = a + from_lane(a, o);
+            if (li == 0) done(u, a);
         }
     }
     if (sh > 6) {                                              // (then there are at most TPB / 128 units)
         __syncthreads();
         if (t < nu) {
-            double a = 0, b = 0;
-            for (int w = 0; w < 1 << (sh - 6); ++w) a += wsum[(t << (sh - 6)) + w].x, b += wsum[(t << (sh - 6)) + w].y;
-            done(t, a, b);
+            E a{};
+            for (int w = 0; w < 1 << (sh - 6); ++w) a = a + wsum[(t << (sh - 6)) + w];
+            done(t, a);
         }
     }
 }
-__device__ __forceinline__ float2 moments(double s1, double s2, double n, float eps) {       // (mean, 1 / sqrt(var + eps))
+// `hold(u)`: where S1 of a unit waits for S2 (8 bytes, the lane's own until then). `rows`: rows in flight that hold anything
+template <int TPB, int V, Sums HOW, typename H, typename F>
+__device__ __forceinline__ void unit_sums(const double (&s1)[kChains<V, HOW>], const double (&s2)[kChains<V, HOW>], int rows, const Lane<V> &l, int nv, int sc, int uw, uint32_t m_uw, uint32_t m_w,
+                                          int nu, void *entries, H hold, F done) {
+    const int W = entries_of(HOW, uw, V);
+    if constexpr (HOW == TURNS) {
+        double *e = (double *)entries;
+        auto put = [&](const double (&v)[V]) {
+            if (l.live)
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (l.owns(j)) e[l.rt * sc + l.lo + j] = v[j];
+            __syncthreads();
+        };
+        auto entry = [&](int u, int r, int c) { return e[r * sc + u * W + c]; };
+        put(s1);
+        add_up<TPB, double>(W, m_w, rows, nu, entry, [&](int u, double a) { *hold(u) = a; });
+        __syncthreads();
+        put(s2);
+        add_up<TPB, double>(W, m_w, rows, nu, entry, [&](int u, double b) { done(u, *hold(u), b); });
+    } else {
+        double2 *e = (double2 *)entries;
+        if constexpr (HOW == EACH) {
+            if (l.live)
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (l.owns(j)) e[l.rt * sc + l.lo + j] = make_double2(s1[j], s2[j]);
+        } else if (l.live) {
+            const int c0 = l.cv * V, next = HOW == ONE ? V : (divided(c0, m_uw) + 1) * uw - l.lo;       // the first channel of the second unit
+            double2 a{}, b{};
+#pragma unroll
+            for (int j = 0; j < kChains<V, HOW>; ++j)
+                if (HOW == ONE || l.owns(j)) {
+                    const double2 v = make_double2(s1[j], s2[j]);
+                    if (HOW == ONE || j < next) a = a + v;
+                    else b = b + v;
+                }
+            e[l.rt * nv + l.cv] = a;
+            if constexpr (HOW == TWO) e[TPB + l.rt * nv + l.cv] = b;
+        }
+        __syncthreads();
+        add_up<TPB, double2>(W, m_w, rows, nu, [&](int u, int r, int c) {
+            if constexpr (HOW == ONE) return e[r * nv + u * W + c];
+            else if constexpr (HOW == EACH) return e[r * sc + u * W + c];
+            else {                                             // the unit's threads; it is the first one's second unit if that one starts before it
+                const int from = u * uw / V, cv = from + c;
+                return cv * V < (u + 1) * uw && cv < nv ? e[(c == 0 && from * V < u * uw ? TPB : 0) + r * nv + cv] : double2{};
+            }
+        }, [&](int u, const double2 &a) { done(u, a.x, a.y); });
+    }
+}
+struct __attribute__((aligned(16))) Moments {
+    float mean, rstd, low;                                    // mean + low: the mean
+};
+__device__ __forceinline__ Moments moments(double s1, double s2, double n, float eps) {       // (one rounding each; NaN stays NaN)
     const double mean = s1 / n, var = s2 / n - mean * mean;
-    return make_float2((float)mean, (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + eps)));        // (one rounding each; NaN stays NaN)
+    const float hi = (float)mean;
+    return Moments{hi, (float)(1.0 / sqrt((var < 0 ? 0.0 : var) + eps)), (float)(mean - hi)};
 }
 
 // ---- split form, first pass: (S1, S2) of each chunk and unit -----------------------------------------------------------------------
-template <typename T, int V, bool ONE>
+template <typename T, int V, Sums HOW>
 __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
     constexpr int TPB = 256, NB = 4;
-    __shared__ __attribute__((aligned(16))) uint8_t entries[kEntryBytes<TPB, V, ONE>];
+    __shared__ __attribute__((aligned(16))) uint8_t entries[entry_bytes(TPB, HOW, V)];
     unsigned id = blockIdx.x;
     const int sl = id % (unsigned)p.nslices;
     id /= (unsigned)p.nslices;
@@ -195,7 +237,7 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
     uint32_t m_nv = p.m_nv, m_w = p.m_w;
     if (sc != p.slice) {                                       // the last slice; the last piece of a group
         nv = (sc + V - 1) / V, m_nv = division_magic(nv);
-        if (p.P > 1) m_w = division_magic(ONE ? uw / V : uw);
+        if (p.P > 1) m_w = division_magic(entries_of(HOW, uw, V));
     }
     const int rp = divided(TPB, m_nv), t = threadIdx.x;
     const Lane<V> l(t, nv, m_nv, rp, sc);
@@ -203,7 +245,16 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
     const T *base = (const T *)p.x + ((int64_t)img * p.R + r0) * p.ldx + s0;
     const int rows = (int)(r1 - r0);
 
-    float n = 0.f, mean[V] = {}, m2[V] = {};
+    constexpr int CH = kChains<V, HOW>;
+    double s1[CH] = {}, s2[CH] = {};
+    auto add = [&](const Pack<T, V> &e) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const double x = to_f32(e.v[j]);
+            s1[j % CH] += x;
+            s2[j % CH] = fma(x, x, s2[j % CH]);
+        }
+    };
     if (l.live) {
         int r = l.rt;
         const T *q = base + (int64_t)r * p.ldx;
@@ -217,41 +268,20 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
             if (r + (2 * NB - 1) * rp < rows)
 #pragma unroll
                 for (int k = 0; k < NB; ++k) nx[k] = load_lane<T, V>(q + k * step, l);
-            const float f = (float)NB * __builtin_amdgcn_rcpf(n + NB), nf = n * f;      // (a weight: its last bit does not matter)
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                float x[NB], m = 0.f, s = 0.f;
-#pragma unroll
-                for (int k = 0; k < NB; ++k) x[k] = to_f32(d[k].v[j]), m += x[k];
-                m *= 1.f / NB;
-#pragma unroll
-                for (int k = 0; k < NB; ++k) s = fmaf(x[k] - m, x[k] - m, s);
-                const float dm = m - mean[j];
-                mean[j] = fmaf(dm, f, mean[j]);
-                m2[j] += fmaf(dm * dm, nf, s);
-            }
-            n += NB;
+            for (int k = 0; k < NB; ++k) add(d[k]);
 #pragma unroll
             for (int k = 0; k < NB; ++k) d[k] = nx[k];
         }
-        for (; r < rows; r += rp, q += step) {
-            const Pack<T, V> e = load_lane<T, V>(q, l);
-            const float f = __builtin_amdgcn_rcpf(n + 1.f), nf = n * f;
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float dm = to_f32(e.v[j]) - mean[j];
-                mean[j] = fmaf(dm, f, mean[j]);
-                m2[j] = fmaf(dm * dm, nf, m2[j]);
-            }
-            n += 1.f;
-        }
+        for (; r < rows; r += rp, q += step) add(load_lane<T, V>(q, l));
     }
     const int per = divided_any(rows, rp), rem = rows - per * rp;
     double2 *out = p.part + ((int64_t)img * p.G * p.P + (p.P == 1 ? divided_any(s0, p.cg) : sl)) * p.S + chunk;
-    unit_sums<TPB, V, ONE>(mean, m2, per, rem, l, nv, rp, sc, uw, m_w, nu, entries, [&](int u, double a, double b) { out[(int64_t)u * p.S] = make_double2(a, b); });
+    unit_sums<TPB, V, HOW>(s1, s2, per > 0 ? rp : rem, l, nv, sc, uw, p.m_uw, m_w, nu, entries, [&](int u) { return &out[(int64_t)u * p.S].x; },
+                           [&](int u, double a, double b) { out[(int64_t)u * p.S] = make_double2(a, b); });
 }
 
-// ---- split form, merge: a workgroup per image and group adds up the chunks and writes (mean, weight / sqrt(var + eps)) of its channels -----
+// ---- split form, merge: a workgroup per image and group adds up the chunks and writes mean, scale and shift of its channels ------------
 __global__ __launch_bounds__(256) void norm_merge_kernel(NormP p) {
     __shared__ double2 red[4];
     const int img = blockIdx.x / (unsigned)p.G, g = blockIdx.x - img * p.G, t = threadIdx.x;
@@ -263,10 +293,13 @@ __global__ __launch_bounds__(256) void norm_merge_kernel(NormP p) {
     a = wave_sum_hi(a), b = wave_sum_hi(b);
     if ((t & 63) == 63) red[t >> 6] = make_double2(a, b);
     __syncthreads();
-    const float2 m = moments((red[0].x + red[1].x) + (red[2].x + red[3].x), (red[0].y + red[1].y) + (red[2].y + red[3].y), (double)p.R * p.cg, p.eps);
+    const Moments m = moments((red[0].x + red[1].x) + (red[2].x + red[3].x), (red[0].y + red[1].y) + (red[2].y + red[3].y), (double)p.R * p.cg, p.eps);
     const int64_t at = (int64_t)img * p.C + g * p.cg;
-    const float *wt = p.w ? p.w + g * p.cg : nullptr;
-    for (int c = t; c < p.cg; c += 256) p.mean[at + c] = m.x, p.scale[at + c] = wt ? m.y * wt[c] : m.y;
+    const float *wt = p.w ? p.w + g * p.cg : nullptr, *bt = p.b ? p.b + g * p.cg : nullptr;
+    for (int c = t; c < p.cg; c += 256) {
+        const float a = wt ? m.rstd * wt[c] : m.rstd;
+        p.mean[at + c] = m.mean, p.scale[at + c] = a, p.shift[at + c] = fmaf(-m.low, a, bt ? bt[c] : 0.f);
+    }
 }
 
 // A thread's V channels of a per-channel array that starts at the slice, as wide loads: one by one each of them touches every line of the row
@@ -287,7 +320,8 @@ template <int V, bool NARROW> __device__ __forceinline__ void load_channels(cons
 
 // ---- normalise, activate, store: shared by both forms -------------------------------------------------------------------------------
 template <int V> struct Affine {
-    float mean[V], a[V], b[V];
+    float mean[V], a[V], b[V];                                // (a, b: weight and bias before `set`)
+    __device__ __forceinline__ void set(int j, const Moments &m) { mean[j] = m.mean, a[j] *= m.rstd, b[j] = fmaf(-m.low, a[j], b[j]); }
 };
 template <typename T, int V> __device__ __forceinline__ void finish(const Pack<T, V> &d, const Affine<V> &f, const NormP &p, float (&y)[V]) {
 #pragma unroll
@@ -336,7 +370,7 @@ __device__ __forceinline__ void store_lane_fp8(uint8_t *qrow, uint8_t *srow, con
     if ((l.cv & 15) == 0) srow[l.cv >> 4] = (uint8_t)byte;
 }
 
-// JOIN: (mean, 1 / sqrt(var + eps)) of the slice's groups from the chunks' sums, here
+// JOIN: the moments of the slice's groups from the chunks' sums, here
 template <typename T, int V, bool TO8, bool JOIN>
 __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int nsl, int S2, int64_t chunk2) {
     constexpr int TPB = 256, NB = TO8 ? 2 : 4;
@@ -350,7 +384,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int
     if (sc != width) nv = threads_of<V, TO8>(sc), m_nv = division_magic(nv);
     const int rp = divided(TPB, m_nv);
     const Lane<V> l(t, nv, m_nv, rp, sc);
-    __shared__ float2 joined[JOIN ? kSliceMax : 1];
+    __shared__ Moments joined[JOIN ? kSliceMax : 1];
     const int first = JOIN ? divided_any(s0, p.cg) : 0;        // the slice's first group
     if constexpr (JOIN) {
         const int ng = divided_any(s0 + sc - 1, p.cg) - first + 1, n = p.S * p.P;
@@ -376,19 +410,19 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int
     uint8_t *oq = TO8 ? p.q + at * p.ldq + s0 : nullptr, *os = TO8 ? p.qs + at * p.ldqs + s0 / kFp8Block : nullptr;
     const int64_t sx = (int64_t)rp * p.ldx;
     Affine<V> f;
-    load_channels<V, TO8>(p.b ? p.b + s0 : nullptr, l, sc, 0.f, f.b);
     if constexpr (JOIN) {
+        load_channels<V, TO8>(p.b ? p.b + s0 : nullptr, l, sc, 0.f, f.b);
         load_channels<V, TO8>(p.w ? p.w + s0 : nullptr, l, sc, 1.f, f.a);
         int g = divided_any(s0 + l.lo, p.cg), in_g = s0 + l.lo - g * p.cg;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float2 st = joined[min(g - first, kSliceMax - 1)];
-            f.mean[j] = st.x, f.a[j] *= st.y;
+            f.set(j, joined[min(g - first, kSliceMax - 1)]);
             if (++in_g == p.cg) in_g = 0, ++g;
         }
     } else {
         load_channels<V, TO8>(p.mean + (int64_t)img * p.C + s0, l, sc, 0.f, f.mean);
         load_channels<V, TO8>(p.scale + (int64_t)img * p.C + s0, l, sc, 0.f, f.a);
+        load_channels<V, TO8>(p.shift + (int64_t)img * p.C + s0, l, sc, 0.f, f.b);
     }
     auto emit = [&](const Pack<T, V> &d, int64_t k) {
         float y[V];
@@ -415,7 +449,7 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormP p, int width, int
 // Rolled loops on purpose: the form serves small maps, whose time is latency, and 50 KB of straight-line code cost more to fetch than the map
 // (27 us for 3 x 1961 x 100 fp16 with the slice in registers and everything unrolled; 8.3 as it is, 8.5 with 4 rows at a time and 10.6 with 8).
 constexpr int kResidentRows = 2; // rows that a thread has under way
-template <typename T, int V, int TPB, bool ONE, bool TO8>
+template <typename T, int V, int TPB, Sums HOW, bool TO8>
 __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
     constexpr int NB = kResidentRows;
     using D = Pack<T, V>;
@@ -426,9 +460,9 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
     id /= (unsigned)p.parts;
     const int sl = id % (unsigned)p.nslices, img = id / (unsigned)p.nslices, t = threadIdx.x;
     const int s0 = sl * p.slice, sc = min(p.slice, p.C - s0), uw = p.cg, mu = divided(p.slice, p.m_uw), nu = divided(sc, p.m_uw);
-    float2 *stat = (float2 *)(dyn + kEntryBytes<TPB, V, ONE>);
+    Moments *stat = (Moments *)(dyn + entry_bytes(TPB, HOW, V));
     constexpr int Q = sizeof(D) / sizeof(W);
-    W *data = (W *)(dyn + kEntryBytes<TPB, V, ONE> + (8 * mu + 15) / 16 * 16) + t;
+    W *data = (W *)(dyn + entry_bytes(TPB, HOW, V) + 16 * mu) + t;
     auto put = [&](W *to, const D &x) {
         W v[Q];
         __builtin_memcpy(v, &x, sizeof(x));
@@ -459,10 +493,8 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
     Affine<V> f;
     load_channels<V, TO8>(p.w ? p.w + s0 : nullptr, l, sc, 1.f, f.a);
     load_channels<V, TO8>(p.b ? p.b + s0 : nullptr, l, sc, 0.f, f.b);
-    // sums of differences to the thread's first row
-    float x0[V], v1[V] = {}, v2[V] = {};
-#pragma unroll
-    for (int j = 0; j < V; ++j) x0[j] = to_f32(d[0].v[j]);
+    constexpr int CH = kChains<V, HOW>;
+    double s1[CH] = {}, s2[CH] = {};
     W *at = data;
     for (int r = l.rt; r < R;) {
 #pragma unroll
@@ -471,9 +503,9 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
             const bool on = r + k * rp < R;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float e = on ? to_f32(d[k].v[j]) - x0[j] : 0.f;
-                v1[j] += e;
-                v2[j] = fmaf(e, e, v2[j]);
+                const double x = on ? to_f32(d[k].v[j]) : 0.f;
+                s1[j % CH] += x;
+                s2[j % CH] = fma(x, x, s2[j % CH]);
             }
         }
         at += NB * Q * TPB;
@@ -481,25 +513,16 @@ __global__ __launch_bounds__(TPB) void norm_resident_kernel(NormP p) {
         if (r < R) load(r);
     }
     const int per = divided_any(R, rp), rem = R - per * rp;
-    const float n = per + (l.rt < rem ? 1 : 0), inv = n > 0.f ? 1.f / n : 0.f;
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float m = v1[j] * inv;
-        v2[j] = fmaf(-v1[j], m, v2[j]);
-        v1[j] = x0[j] + m;
-    }
     Lane<V> le = l;                                            // (the 8-bit form's padding lanes own nothing and take no part in the sums)
     le.live = l.live && l.cv * V < sc;
-    unit_sums<TPB, V, ONE>(v1, v2, per, rem, le, nv, rp, sc, uw, p.m_w, nu, dyn, [&](int u, double a, double b) { stat[u] = moments(a, b, (double)R * uw, p.eps); });
+    unit_sums<TPB, V, HOW>(s1, s2, per > 0 ? rp : rem, le, nv, sc, uw, p.m_uw, p.m_w, nu, dyn, [&](int u) { return (double *)&stat[u]; },
+                           [&](int u, double a, double b) { stat[u] = moments(a, b, (double)R * uw, p.eps); });
     __syncthreads();
     if (!l.live) return;
     int un[V];
-    l.template units<ONE>(uw, p.m_uw, nu, un);
+    l.template units<HOW == ONE>(uw, p.m_uw, nu, un);
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const float2 s = stat[un[j]];
-        f.mean[j] = s.x, f.a[j] *= s.y;
-    }
+    for (int j = 0; j < V; ++j) f.set(j, stat[un[j]]);
     // this workgroup's share of the rows
     const int its = per + (rem ? 1 : 0), share = (its + p.parts - 1) / p.parts, from = part * share, end = min(R, (from + share) * rp);
     at = data + from * (Q * TPB);
@@ -520,7 +543,7 @@ struct NormPlan {
     int V;
     int slice, nslices, P, piece, S;
     int64_t chunk;
-    bool one;
+    Sums sums;
 };
 static int gcd_i(int a, int b) { return b ? gcd_i(b, a % b) : a; }
 constexpr int kMergeMax = 2048;          // chunks x pieces: what one merging workgroup adds up
@@ -538,13 +561,15 @@ static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8)
     const auto last = [&](int64_t w) { return C % w ? C % w : w; };
     if (!to8 && last(slice) < V) V = 1;
     q.V = V;
-    q.one = cg % V == 0;
+    q.sums = sums_of(cg, V);
     const int64_t nv = to8 ? (slice + kFp8Block - 1) / kFp8Block * (kFp8Block / 8) : (slice + V - 1) / V;
     if (nv <= 512 && R <= kResidentBytes) {
         q.tpb = nv <= 256 && R <= 8 * (256 / nv) ? 256 : 512;
         const int64_t rp = q.tpb / nv, its = (R + kResidentRows * rp - 1) / (kResidentRows * rp) * kResidentRows;
         q.slice = (int)slice;
-        q.lds = (size_t)q.tpb * (q.one ? 16 : 8 * V) + (8 * (size_t)(slice / cg) + 15) / 16 * 16 + (size_t)(its * q.tpb * V * es);
+        const size_t map = 16 * (size_t)(slice / cg) + (size_t)(its * q.tpb * V * es);
+        if (q.sums == EACH && entry_bytes(q.tpb, EACH, V) + map > kResidentBytes) q.sums = TURNS;
+        q.lds = entry_bytes(q.tpb, q.sums, V) + map;
         if (q.lds <= kResidentBytes) {
             q.resident = true;
             q.nslices = (int)((C + slice - 1) / slice);
@@ -558,7 +583,7 @@ static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8)
         if (V == 1 || (q.P == 1 ? last(q.slice) : (cg - 1) % q.piece + 1) >= V) break;
     }
     q.V = V;
-    q.one = cg % V == 0;
+    q.sums = sums_of(cg, V);
     // about 4 workgroups per CU, each with at least 8 rows per thread
     const int64_t rp = 256 / ((q.slice + V - 1) / V);
     int64_t S = std::min<int64_t>(1024 / std::max<int64_t>(1, std::min<int64_t>((int64_t)images * q.nslices, 1024)), std::max(1, kMergeMax / q.P));
@@ -570,27 +595,37 @@ static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8)
 }
 
 static int64_t norm_ws(const NormPlan &q, int images, int C, int G) {
-    return q.resident ? 0 : 16 * (int64_t)images * q.S * G * q.P + 8 * (int64_t)images * C;
+    return q.resident ? 0 : 16 * (int64_t)images * q.S * G * q.P + 12 * (int64_t)images * C;
 }
 
-template <typename T, int V, int TPB, bool ONE, bool TO8> static int launch_resident(const NormP &p, const NormPlan &q, int images, hipStream_t s) {
+template <typename T, int V, int TPB, Sums HOW, bool TO8> static int launch_resident(const NormP &p, const NormPlan &q, int images, hipStream_t s) {
     static LdsGrant grant;
     if (q.lds > 64 * 1024)                                       // (all there is, once: two threads' calls never lower each other's limit)
-        if (int rc = grant.ensure((const void *)norm_resident_kernel<T, V, TPB, ONE, TO8>, kResidentBytes, 64 * 1024)) return rc;
+        if (int rc = grant.ensure((const void *)norm_resident_kernel<T, V, TPB, HOW, TO8>, kResidentBytes, 64 * 1024)) return rc;
     NormP n = p;
     const int rp = TPB / threads_of<V, TO8>(q.slice), its = (int)((p.R + rp - 1) / rp);
     n.parts = p.in_place ? 1 : std::max(1, std::min(std::min(12, its), 256 / std::min(256, images * q.nslices)));
     n.nv = threads_of<V, TO8>(q.slice), n.m_nv = division_magic(n.nv);
-    n.m_uw = division_magic(p.cg), n.m_w = division_magic(ONE ? p.cg / V : p.cg);
+    n.m_uw = division_magic(p.cg), n.m_w = division_magic(entries_of(HOW, p.cg, V));
     const int64_t workgroups = (int64_t)images * q.nslices * n.parts;
     LSSVC_CHECK(fits_launch(workgroups, TPB), "group_norm: %lld workgroups do not fit one launch", (long long)workgroups);
-    norm_resident_kernel<T, V, TPB, ONE, TO8><<<(unsigned)workgroups, TPB, q.lds, s>>>(n);
+    norm_resident_kernel<T, V, TPB, HOW, TO8><<<(unsigned)workgroups, TPB, q.lds, s>>>(n);
     return launch_status("group_norm");
 }
 template <typename T, int TPB> static int launch_resident(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {
-    if (to8) return q.one ? launch_resident<T, 8, TPB, true, true>(p, q, images, s) : launch_resident<T, 8, TPB, false, true>(p, q, images, s);
-    if (q.V == 1) return launch_resident<T, 1, TPB, true, false>(p, q, images, s);
-    return q.one ? launch_resident<T, kVecOf<T>, TPB, true, false>(p, q, images, s) : launch_resident<T, kVecOf<T>, TPB, false, false>(p, q, images, s);
+    auto form = [&](auto v, auto to8_) {
+        constexpr int V = decltype(v)::value;
+        constexpr bool TO8 = decltype(to8_)::value;
+        if (q.sums == ONE) return launch_resident<T, V, TPB, ONE, TO8>(p, q, images, s);
+        if constexpr (V > 1) {                                 // (1 divides every width)
+            if (q.sums == TWO) return launch_resident<T, V, TPB, TWO, TO8>(p, q, images, s);
+            if (q.sums == EACH) return launch_resident<T, V, TPB, EACH, TO8>(p, q, images, s);
+        }
+        return launch_resident<T, V, TPB, TURNS, TO8>(p, q, images, s);
+    };
+    if (to8) return form(std::integral_constant<int, 8>{}, std::true_type{});
+    if (q.V == 1) return form(std::integral_constant<int, 1>{}, std::false_type{});
+    return form(std::integral_constant<int, kVecOf<T>>{}, std::false_type{});
 }
 
 template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {
@@ -600,7 +635,7 @@ template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, 
     NormP n = p;
     const int uw = q.P == 1 ? p.cg : q.piece;
     n.nv = q.V == 1 ? q.slice : threads_of<V, false>(q.slice), n.m_nv = division_magic(n.nv);
-    n.m_uw = division_magic(uw), n.m_w = division_magic(q.one ? uw / q.V : uw);
+    n.m_uw = division_magic(uw), n.m_w = division_magic(entries_of(q.sums, uw, q.V));
     // the normalising pass: slices of columns that need not hold whole groups
     const int tail = p.C % kSliceMax, V2 = to8 ? 8 : tail && tail < V ? 1 : V, width = V2 == 1 ? 256 : kSliceMax;
     const int nsl = (p.C + width - 1) / width, sc = std::min(p.C, width);
@@ -613,9 +648,10 @@ template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, 
     const int64_t g2 = images * S2 * nsl;
     const int64_t g_merge = (int64_t)images * p.G;
     LSSVC_CHECK(fits_launch(std::max(std::max(g1, g2), g_merge), 256), "group_norm: %d images of %lld rows do not fit one launch", images, (long long)p.R);
-    if (q.V == 1) norm_stats_kernel<T, 1, true><<<(unsigned)g1, 256, 0, s>>>(n);
-    else if (q.one) norm_stats_kernel<T, V, true><<<(unsigned)g1, 256, 0, s>>>(n);
-    else norm_stats_kernel<T, V, false><<<(unsigned)g1, 256, 0, s>>>(n);
+    if (q.V == 1) norm_stats_kernel<T, 1, ONE><<<(unsigned)g1, 256, 0, s>>>(n);
+    else if (q.sums == ONE) norm_stats_kernel<T, V, ONE><<<(unsigned)g1, 256, 0, s>>>(n);
+    else if (q.sums == TWO) norm_stats_kernel<T, V, TWO><<<(unsigned)g1, 256, 0, s>>>(n);
+    else norm_stats_kernel<T, V, EACH><<<(unsigned)g1, 256, 0, s>>>(n);
     // joining costs every workgroup of the last pass what it reads; a launch costs 3 us of the device's time and as much of the host's
     const bool join = (int64_t)q.S * q.P * p.G <= 1024;
     if (!join) norm_merge_kernel<<<(unsigned)g_merge, 256, 0, s>>>(p);
@@ -694,6 +730,7 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     p.part = (double2 *)workspace;
     p.mean = (float *)(p.part + (int64_t)images * q.S * groups * q.P);
     p.scale = p.mean + (int64_t)images * x->cols;
+    p.shift = p.scale + (int64_t)images * x->cols;
     hipStream_t s = (hipStream_t)stream;
     if (x->dtype == LSSVC_F32) return launch_norm<float>(p, q, images, y8 != nullptr, s);
     if (x->dtype == LSSVC_F16) return launch_norm<f16_t>(p, q, images, y8 != nullptr, s);

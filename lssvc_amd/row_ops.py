@@ -247,8 +247,8 @@ def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
 
 
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None, slope=0.01, images=None, out=None):
-    """act(group_norm(x)): statistics over the rows of each of `images` images and the C / groups channels of a group, in fp32 per thread,
-    joined in 64 bits; weight / bias: C fp32 values. images: for 2-d rows and T (default 1); a 4-d tensor brings its own. out: rows of
+    """act(group_norm(x)): statistics over the rows of each of `images` images and the C / groups channels of a group, sums in 64 bits (finite
+    values of any size and offset); weight / bias: C fp32 values. images: for 2-d rows and T (default 1); a 4-d tensor brings its own. out: rows of
     x's shape and type, x itself allowed. act: None, 'lrelu' (slope), 'relu', 'silu'."""
     return _group_norm(x, groups, weight, bias, eps, act, slope, images, out, False)
 
