@@ -531,6 +531,9 @@ int lssvc_quantize_fp8(const lssvc_rows *x, const lssvc_fp8 *y, void *stream);
  * values or NULL. residual: y's shape and type or NULL; may be y itself. a->rows = 0 is no work. */
 int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const float *bias, int32_t act, float slope, const lssvc_rows *residual,
                      const lssvc_rows *y, void *stream);
+/* Which tile of y (rows x cols per workgroup) that call takes for these operands and this type of results: 16 x 16 ... 64 x 64 share K
+ * among a workgroup's waves, 128 x 128 ... 256 x 256 do not. Looks at sizes, pitches and types only; launches nothing. */
+int lssvc_matmul_fp8_tile(const lssvc_fp8 *a, const lssvc_fp8 *w, int32_t dtype, int32_t *rows, int32_t *cols);
 
 /* Runtime tuning switches (each also reads an environment variable at first use):
  *   "f16x3_persist"            1/0   use the persistent warp-specialised 3x3 kernel (LSSVC_F16X3_PERSIST)

@@ -165,6 +165,7 @@ SIGNATURES = {
     "lssvc_group_norm": (C.c_int, [RP, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_float, C.c_int32, C.c_float, RP, FP, C.c_void_p, C.c_int64, C.c_void_p]),
     "lssvc_quantize_fp8": (C.c_int, [RP, FP, C.c_void_p]),
     "lssvc_matmul_fp8": (C.c_int, [FP, FP, C.c_void_p, C.c_int32, C.c_float, RP, RP, C.c_void_p]),
+    "lssvc_matmul_fp8_tile": (C.c_int, [FP, FP, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "lssvc_set_option": (C.c_int, [C.c_char_p, C.c_int32]),
     "lssvc_get_option": (C.c_int, [C.c_char_p, C.POINTER(C.c_int32)]),
     "lssvc_last_error": (C.c_char_p, []),

@@ -542,22 +542,27 @@ template <int BM, int BN, int WM, int WN, bool E8M0, typename T> static int laun
 // 16-bit and fp32 results, both kinds of scales); the form so chosen takes 0.5 % more than the fastest one in the geometric mean. Split: a start,
 // and for every tile that a CU gets what it reads and an end; where only one workgroup fits a CU, whole rounds of them. Tiles: the
 // same with whole rounds, since a 256 x 256 form's half-empty last round is what the smaller tiles' lower rate is weighed against.
+constexpr int kTile[7][2] = {{16, 16}, {16, 64}, {32, 64}, {64, 64}, {128, 128}, {256, 256}, {192, 256}};      // rows and columns of y per workgroup; 0 - 3: split
+static int choose(const MatmulP &p, bool e8m0) {
+    const bool wide = p.dtype == LSSVC_F32;
+    auto tiles = [&](int i) { return (double)((p.M + kTile[i][0] - 1) / kTile[i][0]) * (double)((p.N + kTile[i][1] - 1) / kTile[i][1]); };
+    auto split = [&](auto form, int i, double start, double read, double widen, double end) {
+        using Form = decltype(form);
+        const double t = tiles(i) / 256, x = 2 * Form::bytes(p.nkb) > 160 * 1024 ? std::ceil(t) : std::max(1.0, t);
+        return start + x * (p.nkb * ((kTile[i][0] + kTile[i][1]) / 16) * read * (wide ? widen : 1.0) + end);
+    };
+    auto tiled = [&](int i, double start, double block, double end) { return start + std::ceil(tiles(i) / 256) * (p.nkb * block + end); };
+    // (a pitch that is no multiple of 128: a block of K straddles two lines)
+    const double pitch = (p.lda | p.ldw) % 128 && p.nkb > 1 ? 1.6 : 1.0, rate = (e8m0 ? 1.0 : 1.17) * pitch, small_rate = (wide ? 2.2 : e8m0 ? 1.0 : 1.2) * pitch;
+    const double cost[7] = {split(Split<1, 1>{}, 0, 2.8, 0.028, 1.25, 0.07), split(Split<1, 4>{}, 1, 3.1, 0.028, 1.38, 0.18),
+                            split(Split<2, 4>{}, 2, 2.9, 0.029, 1.55, 0.9), split(Split<4, 4>{}, 3, 2.6, 0.03, 1.65, 2.4),
+                            tiled(4, 4.3, 0.5 * small_rate, 2.5), wide ? 1e30 : tiled(5, 7.0, 1.38 * rate, 5.0),
+                            wide ? 1e30 : tiled(6, 6.5, 1.1 * rate, 4.0)};
+    return (int)(std::min_element(cost, cost + 7) - cost);
+}
 template <bool E8M0, typename T> static int launch_matmul(const MatmulP &p, hipStream_t s) {
     constexpr bool WIDE = sizeof(T) == 4;
-    auto tiles = [&](int bm, int bn) { return (double)((p.M + bm - 1) / bm) * (double)((p.N + bn - 1) / bn); };
-    auto split = [&](auto form, int mf, int nf, double start, double read, double wide, double end) {
-        using Form = decltype(form);
-        const double t = tiles(16 * mf, 16 * nf) / 256, x = 2 * Form::bytes(p.nkb) > 160 * 1024 ? std::ceil(t) : std::max(1.0, t);
-        return start + x * (p.nkb * (mf + nf) * read * (WIDE ? wide : 1.0) + end);
-    };
-    auto tiled = [&](int bm, int bn, double start, double block, double end) { return start + std::ceil(tiles(bm, bn) / 256) * (p.nkb * block + end); };
-    // (a pitch that is no multiple of 128: a block of K straddles two lines)
-    const double pitch = (p.lda | p.ldw) % 128 && p.nkb > 1 ? 1.6 : 1.0, rate = (E8M0 ? 1.0 : 1.17) * pitch, small_rate = (WIDE ? 2.2 : E8M0 ? 1.0 : 1.2) * pitch;
-    const double cost[7] = {split(Split<1, 1>{}, 1, 1, 2.8, 0.028, 1.25, 0.07), split(Split<1, 4>{}, 1, 4, 3.1, 0.028, 1.38, 0.18),
-                            split(Split<2, 4>{}, 2, 4, 2.9, 0.029, 1.55, 0.9), split(Split<4, 4>{}, 4, 4, 2.6, 0.03, 1.65, 2.4),
-                            tiled(128, 128, 4.3, 0.5 * small_rate, 2.5), WIDE ? 1e30 : tiled(256, 256, 7.0, 1.38 * rate, 5.0),
-                            WIDE ? 1e30 : tiled(192, 256, 6.5, 1.1 * rate, 4.0)};
-    switch (std::min_element(cost, cost + 7) - cost) {
+    switch (choose(p, E8M0)) {
         case 0: return launch_split<1, 1, E8M0, T>(p, s);
         case 1: return launch_split<1, 4, E8M0, T>(p, s);
         case 2: return launch_split<2, 4, E8M0, T>(p, s);
@@ -587,18 +592,39 @@ static int operand_check(const lssvc_fp8 *x, const char *who, int block_rows) {
     LSSVC_CHECK(x->rows < (1LL << 31) - 512 && x->ld < (1LL << 22) && x->scale_ld < (1LL << 21), "matmul_fp8: operand %s is too large", who);
     return 0;
 }
-
-}  // namespace lssvc
-
-using namespace lssvc;
-
-extern "C" int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const float *bias, int32_t act, float slope, const lssvc_rows *residual,
-                                const lssvc_rows *y, void *stream) {
+static int operands_check(const lssvc_fp8 *a, const lssvc_fp8 *w) {
     if (int rc = operand_check(a, "a", 1)) return rc;
     if (int rc = operand_check(w, "w", kFp8Block)) return rc;
     LSSVC_CHECK(w->rows > 0, "matmul_fp8: w has no rows");
     LSSVC_CHECK(a->cols == w->cols, "matmul_fp8: a has %d columns, w has %d", a->cols, w->cols);
     LSSVC_CHECK((a->scale_e8m0 != 0) == (w->scale_e8m0 != 0), "matmul_fp8: one operand has e8m0 scales, the other fp32 scales");
+    return 0;
+}
+static MatmulP operands_of(const lssvc_fp8 *a, const lssvc_fp8 *w, int dtype) {
+    MatmulP p{};
+    p.a = (const uint8_t *)a->values, p.w = (const uint8_t *)w->values;
+    p.sa = a->scale, p.sw = w->scale;
+    p.lda = a->ld, p.ldw = w->ld, p.ldsa = a->scale_ld, p.ldsw = w->scale_ld;
+    p.M = (int)a->rows, p.N = (int)w->rows, p.K16 = (a->cols + 15) / 16 * 16, p.nkb = (a->cols + kFp8Block - 1) / kFp8Block;
+    p.dtype = dtype;
+    return p;
+}
+
+}  // namespace lssvc
+
+using namespace lssvc;
+
+extern "C" int lssvc_matmul_fp8_tile(const lssvc_fp8 *a, const lssvc_fp8 *w, int32_t dtype, int32_t *rows, int32_t *cols) {
+    if (int rc = operands_check(a, w)) return rc;
+    LSSVC_CHECK(rows_type_ok(dtype) && rows && cols, "matmul_fp8_tile: unknown result type %d, or nowhere to put the tile", dtype);
+    const int form = choose(operands_of(a, w, dtype), a->scale_e8m0 != 0);
+    *rows = kTile[form][0], *cols = kTile[form][1];
+    return 0;
+}
+
+extern "C" int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const float *bias, int32_t act, float slope, const lssvc_rows *residual,
+                                const lssvc_rows *y, void *stream) {
+    if (int rc = operands_check(a, w)) return rc;
     LSSVC_CHECK(act_ok(act), "matmul_fp8: unknown activation %d", act);
     if (int rc = rows_check("matmul_fp8", y)) return rc;
     LSSVC_CHECK(y->rows == a->rows && y->cols == w->rows, "matmul_fp8: the output is not %lld x %lld", (long long)a->rows, (long long)w->rows);
@@ -609,14 +635,10 @@ extern "C" int lssvc_matmul_fp8(const lssvc_fp8 *a, const lssvc_fp8 *w, const fl
     if (a->rows == 0) return 0;
     LSSVC_CHECK(!residual || rows_disjoint_or_same(residual, y), "matmul_fp8: residual and output overlap in part");
     LSSVC_CHECK(apart({span_of(y)}, {values_of(a), scales_of(a), values_of(w), scales_of(w), span_of(bias, w->rows)}), "matmul_fp8: the output overlaps an operand or the bias");
-    MatmulP p{};
-    p.a = (const uint8_t *)a->values, p.w = (const uint8_t *)w->values;
-    p.sa = a->scale, p.sw = w->scale;
-    p.lda = a->ld, p.ldw = w->ld, p.ldsa = a->scale_ld, p.ldsw = w->scale_ld;
+    MatmulP p = operands_of(a, w, y->dtype);
     p.bias = bias;
     p.res = residual ? residual->ptr : nullptr, p.ldres = residual ? residual->ld : 0;
     p.y = y->ptr, p.ldy = y->ld;
-    p.M = (int)a->rows, p.N = (int)w->rows, p.K16 = (a->cols + 15) / 16 * 16, p.nkb = (a->cols + kFp8Block - 1) / kFp8Block;
-    p.dtype = y->dtype, p.act = Act{act, slope};
+    p.act = Act{act, slope};
     return a->scale_e8m0 ? launch_typed<true>(p, (hipStream_t)stream) : launch_typed<false>(p, (hipStream_t)stream);
 }

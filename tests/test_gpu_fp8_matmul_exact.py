@@ -1,0 +1,76 @@
+"""The 8-bit product bit for bit: operands whose sums are exact in fp32 in any order, so that a result has one right value, the sum rounded once
+to the output's type, in every tiling and at every number of blocks of K that its loops treat differently."""
+import ctypes as C
+
+import pytest
+import torch
+
+from test_gpu_row_ops import BF16, DEV, F16, F32, ops       # noqa: F401 (ops: fixture)
+
+pytestmark = pytest.mark.gpu
+
+# tile of y -> blocks of K -> rows, columns for which it is chosen, for 16-bit results ("16") and for fp32 ones ("32")
+SHAPES = {
+    ((16, 16), "16"): dict.fromkeys((1, 2, 3, 4, 5, 9, 12, 33), (37, 50)),
+    ((16, 16), "32"): dict.fromkeys((1, 2, 3, 4, 5, 9, 12, 33), (37, 50)),
+    ((16, 64), "16"): {1: (3441, 116), 2: (49, 4607), 3: (49, 4381), 4: (3727, 50), 5: (65, 2892), 9: (3259, 49), 11: (34, 4256), 12: (4034, 34)},
+    ((16, 64), "32"): {1: (3441, 116), 2: (49, 4607), 3: (49, 4381), 4: (3727, 50), 5: (65, 2892), 9: (3259, 49), 11: (34, 4256), 12: (36, 4413)},
+    ((32, 64), "16"): {4: (3974, 87), 5: (3990, 84), 9: (4278, 65), 10: (56, 4486), 11: (4497, 49), 12: (50, 4443)},
+    ((32, 64), "32"): {3: (4248, 101), 4: (4110, 89), 5: (3990, 84), 9: (4278, 65), 10: (81, 3315), 11: (4011, 66), 12: (50, 4978)},
+    ((64, 64), "16"): {4: (4189, 196), 5: (4081, 196), 9: (5006, 134), 10: (4326, 101), 11: (4173, 98), 12: (2848, 149)},
+    ((64, 64), "32"): {4: (3824, 202), 5: (4081, 196), 9: (5006, 134), 10: (116, 4245), 11: (98, 4756), 12: (97, 4867)},
+    ((128, 128), "16"): {1: (4360, 776), 2: (2749, 966), 3: (3415, 667), 4: (3097, 645), 5: (534, 3717), 9: (528, 3603), 10: (647, 2979), 11: (4819, 398), 12: (4685, 404)},
+    ((128, 128), "32"): {1: (4976, 649), 2: (2749, 966), 3: (496, 4874), 4: (2207, 987), 5: (3778, 556), 9: (2912, 719), 10: (2562, 781), 11: (4819, 398), 12: (4685, 404), 33: (4685, 404)},
+    ((192, 256), "16"): {1: (5030, 1551), 2: (3385, 2353), 3: (2311, 3443), 4: (4419, 1804), 5: (1677, 4617), 9: (2338, 3402), 10: (2514, 3243), 11: (3250, 2530), 12: (1747, 4620)},
+    ((256, 256), "16"): {1: (3397, 3685), 2: (4170, 2823), 3: (3773, 3090), 4: (4116, 2824), 5: (3673, 3191), 9: (4428, 2626), 10: (2363, 5016), 11: (3883, 3132), 12: (2516, 4778)},
+}
+CASES = [(tile, m, n, blocks * 128 - cut, out) for (tile, out), at in SHAPES.items() for blocks, (m, n) in at.items() for cut in (0, 40)]
+name = lambda c: "%dx%d-%d-%d-%d-%s" % (c[0] + c[1:])
+
+
+def tile_of(a, w, dtype):
+    from lssvc_amd import _lib
+    rows, cols = C.c_int32(), C.c_int32()
+    _lib.check(_lib.lib.lssvc_matmul_fp8_tile(a._c, w._c, {F32: _lib.F32, F16: _lib.F16, BF16: _lib.BF16}[dtype], C.byref(rows), C.byref(cols)))
+    return rows.value, cols.value
+
+
+def scales(ops, g, values, block_rows, kind, ints, exponents):          # noqa: F811
+    """-> Fp8Rows of `values` with small scales, and the scales as numbers: whole ones in fp32 or powers of two in 8 bits."""
+    shape = (-(-values.shape[0] // block_rows), -(-values.shape[1] // 128))
+    if kind == "any":
+        s = torch.tensor(ints, device=DEV)[torch.randint(len(ints), shape, generator=g, device=DEV)].float()
+        return ops.Fp8Rows(values, s, block_rows), s.double()
+    e = torch.tensor(exponents, device=DEV)[torch.randint(len(exponents), shape, generator=g, device=DEV)]
+    return ops.Fp8Rows(values, (127 + e).to(torch.uint8).view(torch.float8_e8m0fnu), block_rows), torch.exp2(e.double())
+
+
+def numbers(values, scale, block_rows):
+    return values.double() * scale.repeat_interleave(block_rows, 0)[:values.shape[0]].repeat_interleave(128, 1)[:, :values.shape[1]]
+
+
+@pytest.mark.parametrize("kind", ["pow2", "any"])
+@pytest.mark.parametrize("case", CASES, ids=name)
+def test_whole_numbers(ops, case, kind):                                # noqa: F811
+    """Values -4 ... 4, scales 1 ... 4: every product and every sum is a whole number below 2^24, and 16-bit results meet ties. Bias and residual
+    are whole numbers, too."""
+    tile, m, n, k, out = case
+    g = torch.Generator(device=DEV).manual_seed(m + 3 * n + 5 * k)
+    pick = m + n + k // 8
+    dtype = F32 if out == "32" else (F16, BF16)[pick % 2]
+    qa = torch.randint(-4, 5, (m, k), generator=g, device=DEV).to(torch.float8_e4m3fn)
+    qw = torch.randint(-4, 5, (n, k), generator=g, device=DEV).to(torch.float8_e4m3fn)
+    a, sa = scales(ops, g, qa, 1, kind, (1, 2, 3, 4), (0, 1, 2))
+    w, sw = scales(ops, g, qw, 128, kind, (1, 2, 3), (0, 1))
+    assert tile_of(a, w, dtype) == tile
+    a64, w64 = numbers(qa, sa, 1), numbers(qw, sw, 128)
+    assert (a64.abs().amax(0) @ w64.abs().amax(0)) < 2 ** 24            # of any row with any column
+    bias = torch.randint(-50, 51, (n,), generator=g, device=DEV).float()
+    res = torch.randint(-100, 101, (m, n), generator=g, device=DEV).to(dtype) if pick % 3 else None
+    act = (None, "relu", "lrelu")[pick % 3]
+    z = a64 @ w64.t() + bias.double()
+    z = z.clamp(min=0) if act == "relu" else torch.where(z < 0, 0.25 * z, z) if act == "lrelu" else z
+    z = z if res is None else z + res.double()
+    y = ops.matmul_fp8(a, w, bias, act=act, slope=0.25, residual=res, dtype=dtype)
+    assert torch.equal(z.float().double(), z)
+    assert torch.equal(y, z.float().to(dtype))
