@@ -3,9 +3,12 @@
 // 16-bit results: one v_mfma_f32_16x16x128_f8f6f4 covers exactly one block of K, so a block's scales belong to one instruction:
 //   e8m0 scales  the scaled form of the instruction multiplies by 2^(sa + sw) itself; the accumulator runs over all of K.
 //   fp32 scales  each block's product starts from zero and is added to the accumulator with one FMA per value, factor sa * sw.
-// The 8-bit instructions add the products of a group of 8 aligned to the largest of them and drop what lies 13 binary places below its
-// exponent (measured, every 8-bit form does); blocks and groups are added in fp32. For operands that are 8-bit roundings of normal numbers
-// that is 1.3e-5 of the result in the 2-norm: nothing beside half a step of bf16 (2^-8) or fp16 (2^-11), but 200 half steps of fp32.
+// The 8-bit instructions (every form) cut the products of 8 neighbouring columns toward zero at 2^(e - 13), e the largest sum of two operands'
+// exponents among the 8, and add in fp32 from there on: measured, and bit for bit so in the tests. Of the result in the 2-norm that is 1.5e-5 for
+// operands that are 8-bit roundings of normal numbers (K = 1000 ... 50000), 2.1e-5 ... 2.4e-5 where channels differ in spread, 6.7e-5 where one of
+// 8 is 64 times the others, 2.6e-6 (all of it toward zero) where all products are positive. Beside the rounding of bf16 results that is
+// nothing, fp16 results are 0.3 - 5 % further from the exact ones than one rounding would leave them, and fp32 results would be off by hundreds of half
+// steps. Where the large products of a group cancel, what is left may be wrong altogether: a caller whose sums do takes fp32 results.
 // fp32 results: the 8-bit values are widened to fp16, which holds every e4m3 number, and multiplied by v_mfma_f32_16x16x32_f16, which adds in
 // fp32; scales are applied to each block's partial sum. Half the rate, 1e-7.
 // The weights are the instruction's FIRST operand: a lane then holds one row of A (lane & 15) and four consecutive columns of y per

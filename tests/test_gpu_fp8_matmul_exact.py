@@ -74,3 +74,53 @@ def test_whole_numbers(ops, case, kind):                                # noqa: 
     y = ops.matmul_fp8(a, w, bias, act=act, slope=0.25, residual=res, dtype=dtype)
     assert torch.equal(z.float().double(), z)
     assert torch.equal(y, z.float().to(dtype))
+
+
+# ---- what the 8-bit instruction cuts off ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["pow2", "any"])
+@pytest.mark.parametrize("case", [c for c in CASES if c[4] == "16" and c[3] <= 1536], ids=name)
+def test_products_are_cut_as_documented(ops, case, kind):               # noqa: F811
+    """In every 8 columns one has operands of 8 ... 15, the others of 1/8 ... 7.5: the largest sum of exponents is 6 everywhere, all products are cut
+    toward zero at 2^-7, and what is left adds up exactly in any order (multiples of 2^-7 whose magnitudes stay below 2^17). 96 rows and columns, spread
+    over the result."""
+    tile, m, n, k, _ = case
+    g = torch.Generator(device=DEV).manual_seed(m + n + k)
+    dtype = (F16, BF16)[(m + k // 8) % 2]
+    at = torch.arange(k, device=DEV)
+    large = at % 8 == at // 8 % 8
+
+    def values(rows):
+        e = torch.where(large, 3, torch.randint(-3, 3, (rows, k), generator=g, device=DEV))
+        v = torch.exp2(e.float()) * (1 + torch.randint(0, 8, (rows, k), generator=g, device=DEV) / 8)
+        return (v * (1 - 2 * torch.randint(0, 2, (rows, k), generator=g, device=DEV))).to(torch.float8_e4m3fn)
+    qa, qw = values(m), values(n)
+    a, sa = scales(ops, g, qa, 1, kind, (1, 3), (0, 1))
+    w, sw = scales(ops, g, qw, 128, kind, (1,), (0, 1))
+    assert tile_of(a, w, dtype) == tile
+    rows, cols = torch.randperm(m, generator=g, device=DEV)[:96], torch.randperm(n, generator=g, device=DEV)[:96]
+    p = qa[rows].double()[:, None] * qw[cols].double()[None]
+    scale = sa[rows][:, None] * sw[cols // 128][None]
+    cut = (torch.trunc(p * 128) / 128) * scale.repeat_interleave(128, 2)[:, :, :k]
+    assert cut.abs().sum(2).max() < 2 ** 17
+    z = cut.sum(2)
+    y = ops.matmul_fp8(a, w, dtype=dtype)[rows][:, cols]
+    assert torch.equal(y, z.float().to(dtype))
+
+
+@pytest.mark.parametrize("m", [5, 700])
+def test_where_large_products_cancel(ops, m):                           # noqa: F811
+    """256 - 256 + 7 small products: 16-bit results lose the small ones of the same 8 columns from 2^-13 of the large one down, and keep those of
+    others; fp32 results lose nothing."""
+    a = torch.zeros(m, 272, device=DEV)
+    a[:, 3], a[:, 256] = 256, -256
+    a[:, 0:3] = 2.0 ** -6
+    near = ops.quantize_fp8(a)
+    a[:, 0:3], a[:, 16:19] = 0, 2.0 ** -6
+    far = ops.quantize_fp8(a)
+    a[:, 16:19], a[:, 0:3] = 0, 2.0 ** -5
+    kept = ops.quantize_fp8(a)
+    w = ops.quantize_fp8(torch.ones(600, 272, device=DEV), 128)
+    for dtype in (F16, BF16, F32):
+        sums = [ops.matmul_fp8(q, w, dtype=dtype).float() for q in (near, far, kept)]
+        want = (0.0 if dtype != F32 else 3 * 2.0 ** -6, 3 * 2.0 ** -6, 3 * 2.0 ** -5)
+        assert all((s == v).all() for s, v in zip(sums, want)), dtype
