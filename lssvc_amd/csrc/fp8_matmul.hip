@@ -412,8 +412,9 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void matmul_tile_kernel
     constexpr bool BY_PART = !E8M0 || WIDE;
     f32x4 late = {0.f, 0.f, 0.f, 0.f};
     float late_scale = 0.f;
-    // one block of K; S = kb % 4. No branches inside: the compiler would gather the products behind them. (A block behind the last one is filled
-    // with zeros, its descriptor's range being empty, and read for nothing.)
+    // one block of K; S = kb % 4. No branches inside: the compiler would gather the products behind them. (Behind the last block the look-ahead
+    // loads that block again; its fragments are read and never multiplied. Such loads are still on their way into the LDS when the loop ends: the
+    // wait and the barrier before the epilogue are what lets it use that memory.)
     auto step = [&](int kb, auto s_) {
         constexpr int S = decltype(s_)::value;
         Frag<WIDE> wf[FN];
