@@ -12,11 +12,14 @@ Rows are given as one of
     torch.Tensor (rows, C)                      any pitch between rows, channels adjacent
     torch.Tensor (N, C, H, W)                   torch.channels_last memory, or a channel slice of such a tensor
 and come back as the same kind. Everything is enqueued on the current stream of the tensors' device; nothing synchronises. The
-operators are forward operators (a tensor that requires a gradient is refused) and are not part of compiled frame plans.
+operators are forward operators: a tensor that requires a gradient or carries a forward-mode tangent is refused, and so is a call inside
+torch.jit.trace, make_fx or a torch.func transform. They are not part of compiled frame plans.
 """
 import functools
+import sys
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, hip_ops
 from ._lib import LssvcHipError, Rows, Fp8, check, lib
@@ -36,6 +39,13 @@ def _refuse(what, *args):
 def _no_grad(x, name):
     if x.requires_grad and torch.is_grad_enabled():
         _refuse("row_ops: %s requires a gradient and these operators have none (use torch.no_grad() or detach())", name)
+
+
+def _no_tangent(*tensors):
+    """For calls inside a level of forward-mode differentiation, where x.requires_grad says nothing."""
+    for x in tensors:
+        if isinstance(x, torch.Tensor) and forward_ad.unpack_dual(x).tangent is not None:
+            _refuse("row_ops: a tensor carries a forward-mode tangent and these operators have no derivative")
 
 
 def _rows(x, name):
@@ -95,8 +105,24 @@ def _act_code(act):
 _raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _elsewhere(device):
-    """Whether `device` has to be made current for a call (every entry point does that around itself)."""
+# who else may be watching: a trace or transform sees a call's allocations and not its launches, and what it makes of them would be wrong without an
+# error. (All four looks together: 0.2 us.)
+_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+_transform = getattr(getattr(torch._C, "_functorch", None), "peek_interpreter_stack", lambda: None)
+_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+
+
+def _no_proxies():
+    proxies = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    return proxies is None or proxies.get_proxy_mode() is None
+
+
+def _elsewhere(device, *tensors):
+    """Whether `device` has to be made current for a call (every entry point does that around itself). tensors: the call's."""
+    if _tracing() or _transform() is not None or _modes() and not _no_proxies():
+        _refuse("row_ops: these operators cannot be traced or transformed (torch.jit.trace, make_fx, torch.func)")
+    if getattr(forward_ad, "_current_level", 0) >= 0:              # (not known: look)
+        _no_tangent(*tensors)
     if hip_ops.PLAN_RECORDER is not None:
         _refuse("row_ops: not part of compiled frame plans")
     return device.index != _current_device()
@@ -125,6 +151,8 @@ class Fp8Rows:
         if not 1 <= cols <= _MAX_COLS or tuple(scale.shape) != want:
             _refuse("Fp8Rows: scale is %s, expected %s for %d x %d values in %d x %d blocks", tuple(scale.shape), want, rows, cols, block_rows, BLOCK)
         _no_grad(scale, "scale")
+        _no_grad(values, "values")
+        _no_tangent(scale, values)
         if rows and not (cols % 16 == 0 and values.stride(1) == 1 and (rows == 1 or values.stride(0) % 16 == 0 and values.stride(0) >= cols) and values.data_ptr() % 16 == 0):
             values = _padded(values, _pitch(cols))
         if rows and scale.dtype == _E8M0 and not (want[1] % 4 == 0 and scale.stride(1) == 1 and scale.data_ptr() % 4 == 0
@@ -211,7 +239,7 @@ _norm_workspace = functools.lru_cache(1024)(lib.lssvc_group_norm_workspace_bytes
 def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
     dev = x.device if isinstance(x, (T, torch.Tensor)) else None
     xr = _rows(x, "x")
-    if _elsewhere(dev):
+    if _elsewhere(dev, x, weight, bias, out):
         with torch.cuda.device(dev):
             return _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8)
     if images is None:
@@ -264,7 +292,7 @@ def quantize_fp8(x, block_rows=1, out=None):
     finite becomes NaN and does not move the scale."""
     xr = _rows(x, "x")
     dev = x.device
-    if _elsewhere(dev):
+    if _elsewhere(dev, x):
         with torch.cuda.device(dev):
             return quantize_fp8(x, block_rows, out)
     out = _fp8_out(out, xr.rows, xr.cols, dev, block_rows)
@@ -287,7 +315,7 @@ def matmul_fp8(a, w, bias=None, *, act=None, slope=0.01, residual=None, out=None
     if not isinstance(a, Fp8Rows) or not isinstance(w, Fp8Rows):
         _refuse("matmul_fp8: operands are Fp8Rows (quantize_fp8, group_norm_fp8)")
     dev = a.device
-    if _elsewhere(dev):
+    if _elsewhere(dev, bias, residual, out):
         with torch.cuda.device(dev):
             return matmul_fp8(a, w, bias, act=act, slope=slope, residual=residual, out=out, dtype=dtype)
     m, n = a.rows, w.rows

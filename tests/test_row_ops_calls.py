@@ -1,0 +1,53 @@
+"""Calls that torch would follow only in part are refused: no GPU needed."""
+import pytest
+import torch
+
+
+@pytest.fixture
+def here(monkeypatch):
+    """What every operator asks first, on a machine without a GPU."""
+    from lssvc_amd import row_ops
+    monkeypatch.setattr(row_ops, "_current_device", lambda: 0)
+    return lambda: row_ops._elsewhere(torch.device("cuda:0"))
+
+
+def test_traces_and_transforms_are_refused(here):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from lssvc_amd.row_ops import LssvcHipError
+    assert here() is False
+    x, calls = torch.randn(2, 3), []
+
+    def f(x):
+        calls.append(1)
+        here()
+        return x.sum()
+    for run in (lambda: torch.jit.trace(f, x), lambda: make_fx(f)(x), lambda: torch.func.vmap(f)(x), lambda: torch.func.grad(f)(x), lambda: torch.func.jvp(f, (x,), (x,)),
+                lambda: torch.func.functionalize(f)(x)):
+        n = len(calls)
+        with pytest.raises(LssvcHipError, match="traced or transformed"):
+            run()
+        assert len(calls) > n
+    from torch.utils.flop_counter import FlopCounterMode
+    with FlopCounterMode(display=False):                              # a mode that records nothing is no hindrance
+        assert here() is False
+    assert here() is False
+
+
+def test_derivatives_are_refused_in_both_modes(here):
+    from torch.autograd import forward_ad
+    from lssvc_amd import row_ops
+    x = torch.randn(3, 4)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        ask = lambda *tensors: row_ops._elsewhere(torch.device("cuda:0"), *tensors)
+        assert ask(x, None, forward_ad.unpack_dual(d).primal) is False
+        for others in ((d,), (x, None, d)):
+            with pytest.raises(row_ops.LssvcHipError, match="tangent"):
+                ask(*others)
+        with torch.no_grad(), pytest.raises(row_ops.LssvcHipError, match="tangent"):       # (which leaves forward mode on)
+            ask(d)
+    x.requires_grad_()
+    with pytest.raises(row_ops.LssvcHipError, match="gradient"):
+        row_ops._no_grad(x, "x")
+    with torch.no_grad():
+        row_ops._no_grad(x, "x")
