@@ -89,7 +89,7 @@ class _Branch:
             self.outer_keep, self.outer_fork = _TLS.keep, _TLS.fork
             s = f.streams[self.i]
             s.wait_stream(torch.cuda.current_stream())
-            if PLAN_RECORDER is not None:
+            if recording():
                 PLAN_RECORDER.wait(s.cuda_stream, torch.cuda.current_stream().cuda_stream)
             self.ctx = torch.cuda.stream(s)
             self.ctx.__enter__()
@@ -128,7 +128,7 @@ class Fork:
         assert _TLS.keep is None or _TLS.fork is not self, "join from the forking stream, not from inside a branch of the same Fork"
         if self.enabled and i in self.open:
             torch.cuda.current_stream().wait_stream(self.streams[i])
-            if PLAN_RECORDER is not None:
+            if recording():
                 PLAN_RECORDER.wait(torch.cuda.current_stream().cuda_stream, self.streams[i].cuda_stream)
             self.open.discard(i)
             done = self.keep.pop(i, None)          # the joining stream has waited for the branch: its buffers may be recycled ...
@@ -201,6 +201,12 @@ ARENA = None                  # plan_compiler.Arena while a frame plan is being 
 PLAN_RECORDER = None          # plan_compiler.Recorder while a frame plan is being recorded (fork / join edges are reported to it)
 
 
+def recording():
+    """Whether THIS thread is recording a frame plan: other threads' launches and buffers have no part in it."""
+    rec = PLAN_RECORDER
+    return rec is not None and rec.thread == _threading.get_ident()
+
+
 class T:
     """An H x W x C fp32 view (batch 1) with pixel pitch `ld` into a flat torch buffer."""
     __slots__ = ("buf", "H", "W", "C", "ld", "off", "_v", "split")
@@ -212,7 +218,7 @@ class T:
 
     @staticmethod
     def empty(H, W, Cc, device):
-        if ARENA is not None:                    # a frame plan is being compiled (plan_compiler.py): activations from ONE arena
+        if recording():                          # a frame plan is being compiled (plan_compiler.py): activations from ONE arena
             return T(ARENA.alloc_f32(H * W * Cc), H, W, Cc, Cc)
         if GUARD_EMPTY:              # debugging aid: every activation buffer between two sentinel zones, checked by check_guards()
             G = 1024
@@ -646,7 +652,7 @@ def presplit(x, in_act=None, in_slope=0.01, out=None):
     """fp32 view -> pre-split view (fp16 hi | lo per 16-channel chunk, the input activation applied): lssvc_presplit."""
     if out is None:
         cp = (x.C + 15) // 16 * 16
-        if ARENA is not None:
+        if recording():
             out = T(ARENA.alloc_f32(x.H * x.W * cp), x.H, x.W, x.C, cp, split=True)
         else:
             out = T(torch.empty(x.H * x.W * cp, dtype=torch.float32, device=x.device), x.H, x.W, x.C, cp, split=True)

@@ -19,6 +19,7 @@ that runs once per (checkpoint, frame size); a plan is specific to that pair, li
 """
 import ctypes as C
 import struct
+import threading
 import weakref
 
 import torch
@@ -98,6 +99,7 @@ class Recorder:
     def __init__(self, device, arena_bytes, weight_stores, scratch, inputs, outputs):
         """scratch / inputs / outputs: {name: tensor}; weight_stores: the models' WeightStore objects."""
         self.device = device
+        self.thread = None        # the thread that records (between __enter__ and __exit__): other threads' launches are not the plan's
         self.arena = Arena(arena_bytes, device)
         self.regions = [{"kind": REGION_ARENA, "name": "arena", "ptr": self.arena.buf.data_ptr(), "nbytes": self.arena.buf.numel(), "data": None}]
         for kind, group in ((REGION_SCRATCH, scratch), (REGION_INPUT, inputs), (REGION_OUTPUT, outputs)):
@@ -209,10 +211,13 @@ class Recorder:
             self._orig[name] = fn
 
             def wrapper(*args, _fn=fn, _name=name):
+                if threading.get_ident() != self.thread:
+                    return _fn(*args)
                 stream, enc = self._encode(_name, args)
                 self.launches.append((_name, stream, enc))
                 return _fn(*args)
             setattr(lib, name, wrapper)
+        self.thread = threading.get_ident()
         ops.ARENA = self.arena
         ops.PLAN_RECORDER = self
         return self
@@ -222,6 +227,7 @@ class Recorder:
             setattr(_lib.lib, name, fn)
         ops.ARENA = None
         ops.PLAN_RECORDER = None
+        self.thread = None
         return False
 
     # ---- file ------------------------------------------------------------------------------------------------------

@@ -123,7 +123,7 @@ def _elsewhere(device, *tensors):
         _refuse("row_ops: these operators cannot be traced or transformed (torch.jit.trace, make_fx, torch.func)")
     if getattr(forward_ad, "_current_level", 0) >= 0:              # (not known: look)
         _no_tangent(*tensors)
-    if hip_ops.PLAN_RECORDER is not None:
+    if hip_ops.recording():
         _refuse("row_ops: not part of compiled frame plans")
     return device.index != _current_device()
 

@@ -51,3 +51,35 @@ def test_derivatives_are_refused_in_both_modes(here):
         row_ops._no_grad(x, "x")
     with torch.no_grad():
         row_ops._no_grad(x, "x")
+
+
+def test_a_plan_is_recorded_from_its_own_thread_only(here):
+    """One thread records a frame plan: its own row operators are refused, another thread's launches and buffers are left alone."""
+    import ctypes as C
+    import threading
+    from lssvc_amd import _lib, hip_ops
+    from lssvc_amd.plan_compiler import Recorder
+    cpu = torch.device("cpu")
+    bad = lambda: _lib.lib.lssvc_fill_zero(C.c_void_p(None), 4, C.c_void_p(None))        # refused on the host, wherever it is called
+    got = {}
+
+    def other():
+        got["elsewhere"] = here()
+        got["status"] = bad()
+        t = hip_ops.T.empty(2, 2, 4, cpu)
+        got["in arena"] = rec.arena.buf.data_ptr() <= t.buf.data_ptr() < rec.arena.buf.data_ptr() + rec.arena.buf.numel()
+        got["recording"] = hip_ops.recording()
+    rec = Recorder(cpu, 1 << 16, [], {}, {}, {})
+    with rec:
+        assert hip_ops.recording()
+        with pytest.raises(_lib.LssvcHipError, match="frame plans"):
+            here()
+        t = hip_ops.T.empty(2, 2, 4, cpu)
+        assert rec.arena.buf.data_ptr() <= t.buf.data_ptr() < rec.arena.buf.data_ptr() + rec.arena.buf.numel()
+        thread = threading.Thread(target=other)
+        thread.start()
+        thread.join()
+        assert rec.launches == []
+        assert bad() != 0 and len(rec.launches) == 1
+    assert got == {"elsewhere": False, "status": got["status"], "in arena": False, "recording": False} and got["status"] != 0
+    assert not hip_ops.recording() and here() is False
