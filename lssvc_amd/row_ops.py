@@ -118,7 +118,11 @@ def _no_proxies():
 
 
 def _elsewhere(device, *tensors):
-    """Whether `device` has to be made current for a call (every entry point does that around itself). tensors: the call's."""
+    """Whether `device` has to be made current for a call (every entry point does that around itself). tensors: what the caller gave; in a branch of
+    hip_ops.Fork they are alive until it is joined, as the engine's views are."""
+    keep = hip_ops._TLS.keep
+    if keep is not None:
+        keep.extend(tensors)
     if _tracing() or _transform() is not None or _modes() and not _no_proxies():
         _refuse("row_ops: these operators cannot be traced or transformed (torch.jit.trace, make_fx, torch.func)")
     if getattr(forward_ad, "_current_level", 0) >= 0:              # (not known: look)
@@ -292,7 +296,7 @@ def quantize_fp8(x, block_rows=1, out=None):
     finite becomes NaN and does not move the scale."""
     xr = _rows(x, "x")
     dev = x.device
-    if _elsewhere(dev, x):
+    if _elsewhere(dev, x, out):
         with torch.cuda.device(dev):
             return quantize_fp8(x, block_rows, out)
     out = _fp8_out(out, xr.rows, xr.cols, dev, block_rows)
@@ -315,7 +319,7 @@ def matmul_fp8(a, w, bias=None, *, act=None, slope=0.01, residual=None, out=None
     if not isinstance(a, Fp8Rows) or not isinstance(w, Fp8Rows):
         _refuse("matmul_fp8: operands are Fp8Rows (quantize_fp8, group_norm_fp8)")
     dev = a.device
-    if _elsewhere(dev, bias, residual, out):
+    if _elsewhere(dev, a, w, bias, residual, out):
         with torch.cuda.device(dev):
             return matmul_fp8(a, w, bias, act=act, slope=slope, residual=residual, out=out, dtype=dtype)
     m, n = a.rows, w.rows

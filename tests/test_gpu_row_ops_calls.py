@@ -30,3 +30,32 @@ def test_derivatives_and_traces_are_refused(ops):          # noqa: F811
         ops.Fp8Rows(values, q.scale)
     with torch.no_grad():
         assert ops.Fp8Rows(values, q.scale).rows == 32
+
+
+def test_a_branch_keeps_what_it_reads_until_it_is_joined(ops):      # noqa: F811
+    """Inputs that the caller drops while a branch on a side stream still reads them: their memory goes to nobody else before the join."""
+    import gc
+    import weakref
+    from lssvc_amd.hip_ops import Fork
+    g = gen(3)
+    x, b = torch.randn(4000, 64, generator=g).to(DEV), torch.randn(64, generator=g).to(DEV)
+    want = ops.group_norm(x, 4, None, b)
+    w = ops.quantize_fp8(torch.randn(64, 64, generator=g).to(DEV), 128)
+    q = ops.quantize_fp8(want)
+    want = ops.matmul_fp8(q, w, b, residual=want)
+    fork = Fork(torch.device(DEV), enabled=True, tag="row_ops")
+    x, b, w = x.clone(), b.clone(), ops.quantize_fp8(w.dequantize(), 128)
+    refs = [weakref.ref(x), weakref.ref(b), weakref.ref(w.values)]
+    with fork.branch(0):
+        y = ops.group_norm(x, 4, None, b)
+        q = ops.quantize_fp8(y)
+        refs.append(weakref.ref(y))
+        y = ops.matmul_fp8(q, w, b, residual=y)
+        del x, b, w, q
+    gc.collect()
+    assert all(r() is not None for r in refs)
+    noise = [torch.full((4000, 64), float("nan"), device=DEV) for _ in range(4)]       # what would get the memory
+    fork.join(0)
+    gc.collect()
+    assert all(r() is None for r in refs)
+    assert torch.equal(y, want) and len(noise) == 4
