@@ -16,6 +16,7 @@ operators are forward operators: a tensor that requires a gradient or carries a 
 torch.jit.trace, make_fx or a torch.func transform. They are not part of compiled frame plans.
 """
 import functools
+import operator
 import sys
 
 import torch
@@ -93,8 +94,26 @@ def _vector(x, name, n, device):
     return x.data_ptr()
 
 
+def _whole(v, name):
+    try:
+        return operator.index(v)
+    except TypeError:
+        _refuse("row_ops: %s has to be a whole number, got %r", name, v)
+
+
+def _number(v, name):
+    if isinstance(v, torch.Tensor):
+        _refuse("row_ops: %s has to be a number, not a tensor (which would have to be waited for)", name)
+    try:
+        if not isinstance(v, str):
+            return float(v)
+    except (TypeError, ValueError):
+        pass
+    _refuse("row_ops: %s has to be a number, got %r", name, v)
+
+
 def _act_code(act):
-    code = _ACT.get(act)
+    code = _ACT.get(act) if act is None or isinstance(act, str) else None
     if code is None:
         _refuse("row_ops: unknown activation %r (None, 'lrelu', 'relu', 'silu')", act)
     return code
@@ -129,6 +148,8 @@ def _elsewhere(device, *tensors):
         _no_tangent(*tensors)
     if hip_ops.recording():
         _refuse("row_ops: not part of compiled frame plans")
+    if device.index is None:
+        _refuse("row_ops: 8-bit rows on %s: there is no CPU path", device)
     return device.index != _current_device()
 
 
@@ -148,6 +169,7 @@ class Fp8Rows:
             _refuse("Fp8Rows: values have to be a (rows, cols) torch.float8_e4m3fn tensor on the GPU")
         if not isinstance(scale, torch.Tensor) or scale.dtype not in (_E8M0, torch.float32) or scale.dim() != 2 or scale.device != values.device:
             _refuse("Fp8Rows: scale has to be a 2-d torch.float8_e8m0fnu or torch.float32 tensor on the values' device")
+        block_rows = _whole(block_rows, "block_rows")
         if block_rows not in (1, BLOCK):
             _refuse("Fp8Rows: block_rows is 1 or %d, got %r", BLOCK, block_rows)
         rows, cols = values.shape
@@ -192,6 +214,7 @@ class Fp8Rows:
     @staticmethod
     def empty(rows, cols, device, block_rows=1):
         """Uninitialised rows with e8m0 scales, for `out=` of the operators that write 8-bit rows."""
+        rows, cols, block_rows = _whole(rows, "rows"), _whole(cols, "cols"), _whole(block_rows, "block_rows")
         if block_rows != 1 and block_rows != BLOCK:
             _refuse("Fp8Rows: block_rows is 1 or %d, got %r", BLOCK, block_rows)
         if rows < 0 or not 1 <= cols <= _MAX_COLS:
@@ -243,6 +266,12 @@ _norm_workspace = functools.lru_cache(1024)(lib.lssvc_group_norm_workspace_bytes
 def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
     dev = x.device if isinstance(x, (T, torch.Tensor)) else None
     xr = _rows(x, "x")
+    if groups.__class__ is not int:
+        groups = _whole(groups, "groups")
+    if images is not None and images.__class__ is not int:
+        images = _whole(images, "images")
+    if eps.__class__ is not float or slope.__class__ is not float:
+        eps, slope = _number(eps, "eps"), _number(slope, "slope")
     if _elsewhere(dev, x, weight, bias, out):
         with torch.cuda.device(dev):
             return _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8)
@@ -324,12 +353,14 @@ def matmul_fp8(a, w, bias=None, *, act=None, slope=0.01, residual=None, out=None
             return matmul_fp8(a, w, bias, act=act, slope=slope, residual=residual, out=out, dtype=dtype)
     m, n = a.rows, w.rows
     code = _act_code(act)
+    if slope.__class__ is not float:
+        slope = _number(slope, "slope")
     bp = None if bias is None else _vector(bias, "bias", n, dev)
     rr = None if residual is None else _rows(residual, "residual")
     if out is None:
         if dtype is None:
             dtype = torch.bfloat16 if rr is None else torch.float32 if isinstance(residual, T) else residual.dtype
-        dt = _DTYPE.get(dtype)
+        dt = _DTYPE.get(dtype) if isinstance(dtype, torch.dtype) else None
         if dt is None:
             _refuse("matmul_fp8: type %s (fp32, fp16 or bf16 expected)", dtype)
         if rr is None or (not isinstance(residual, T) and residual.dim() == 2):
@@ -340,7 +371,7 @@ def matmul_fp8(a, w, bias=None, *, act=None, slope=0.01, residual=None, out=None
             yr = _rows(out, "out")
     else:
         yr = _rows(out, "out")
-    if dtype is not None and _DTYPE.get(dtype) != yr.dtype:
+    if dtype is not None and not (isinstance(dtype, torch.dtype) and _DTYPE.get(dtype) == yr.dtype):
         _refuse("matmul_fp8: dtype %s is not the output's", dtype)
     if w.device != dev or residual is not None and residual.device != dev or out.device != dev:
         _refuse("matmul_fp8: operands on several devices")

@@ -59,3 +59,22 @@ def test_a_branch_keeps_what_it_reads_until_it_is_joined(ops):      # noqa: F811
     gc.collect()
     assert all(r() is None for r in refs)
     assert torch.equal(y, want) and len(noise) == 4
+
+
+def test_arguments_of_other_types(ops):          # noqa: F811
+    """Numbers of any kind are taken; what is none is refused with the operators' own error."""
+    import numpy as np
+    x = torch.randn(32, 64, device=DEV)
+    q, w = ops.quantize_fp8(x), ops.quantize_fp8(torch.randn(48, 64, device=DEV), 128)
+    y = ops.group_norm(x, 4, eps=1.0, act="lrelu", slope=2.0, images=2)
+    assert torch.equal(y, ops.group_norm(x, np.int32(4), eps=1, act="lrelu", slope=np.float32(2), images=np.int64(2)))
+    for call in (lambda: ops.group_norm(x, 4.0), lambda: ops.group_norm(x, None), lambda: ops.group_norm(x, "4"), lambda: ops.group_norm(x, 4, images=1.5),
+                 lambda: ops.group_norm(x, 4, eps=None), lambda: ops.group_norm(x, 4, eps=torch.tensor(1e-5, device=DEV)), lambda: ops.group_norm(x, 4, act=[]),
+                 lambda: ops.group_norm(x, 4, slope="0.1"), lambda: ops.group_norm_fp8(x, 4.0), lambda: ops.quantize_fp8(x, 1.0), lambda: ops.quantize_fp8(x, None),
+                 lambda: ops.matmul_fp8(q, w, slope=None), lambda: ops.matmul_fp8(q, w, act=1), lambda: ops.matmul_fp8(q, w, dtype="bf16"), lambda: ops.matmul_fp8(q, w, dtype=[]),
+                 lambda: ops.matmul_fp8(q, w, out=torch.empty(32, 48, device=DEV), dtype=[]), lambda: ops.matmul_fp8(ops.Fp8Rows.empty(32, 64, "cpu"), w),
+                 lambda: ops.matmul_fp8(q, ops.Fp8Rows.empty(48, 64, "cpu", 128)), lambda: ops.quantize_fp8(x, out=ops.Fp8Rows.empty(32, 64, "cpu")),
+                 lambda: ops.Fp8Rows(q.values, q.scale, 1.0)):
+        with pytest.raises(ops.LssvcHipError):
+            call()
+    assert torch.equal(ops.group_norm(x, 4, eps=1.0, act="lrelu", slope=2.0, images=2), y)

@@ -83,3 +83,17 @@ def test_a_plan_is_recorded_from_its_own_thread_only(here):
         assert bad() != 0 and len(rec.launches) == 1
     assert got == {"elsewhere": False, "status": got["status"], "in arena": False, "recording": False} and got["status"] != 0
     assert not hip_ops.recording() and here() is False
+
+
+def test_arguments_of_other_types_are_refused_by_name(here):
+    from lssvc_amd import row_ops
+    E, rows = row_ops.LssvcHipError, row_ops.Fp8Rows.empty
+    a, w = rows(8, 64, "cpu"), rows(16, 64, "cpu", 128)
+    for call, text in ((lambda: row_ops.matmul_fp8(a, w), "no CPU path"), (lambda: row_ops._act_code([]), "activation"), (lambda: row_ops._act_code(1), "activation"),
+                       (lambda: row_ops._whole(4.0, "groups"), "groups"), (lambda: row_ops._whole("4", "images"), "images"), (lambda: row_ops._number(None, "eps"), "eps"),
+                       (lambda: row_ops._number("a", "slope"), "slope"), (lambda: row_ops._number("0.1", "slope"), "slope"), (lambda: row_ops._number(torch.tensor(1e-5), "eps"), "tensor"),
+                       (lambda: rows(8, 64, "cpu", 1.0), "block_rows"), (lambda: rows(8.0, 64, "cpu"), "rows"), (lambda: rows(8, None, "cpu"), "cols")):
+        with pytest.raises(E, match=text):
+            call()
+    import numpy as np
+    assert row_ops._whole(np.int64(4), "groups") == 4 and row_ops._number(1, "eps") == 1.0 and row_ops._number(np.float32(0.5), "slope") == 0.5
