@@ -120,8 +120,9 @@ def _act_code(act):
 
 
 # torch.cuda.current_stream(device).cuda_stream without the Stream object, torch.cuda.current_device() without its look at whether the GPU is in
-# use already (a tensor on it says so): 1.3 us of a call's 6 to 8
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+# use already (a tensor on it says so): 1.3 us of a call's 6 to 8. Both are names inside torch: a torch without them has the public ones.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 # who else may be watching: a trace or transform sees a call's allocations and not its launches, and what it makes of them would be wrong without an

@@ -78,3 +78,14 @@ def test_arguments_of_other_types(ops):          # noqa: F811
         with pytest.raises(ops.LssvcHipError):
             call()
     assert torch.equal(ops.group_norm(x, 4, eps=1.0, act="lrelu", slope=2.0, images=2), y)
+
+
+def test_on_a_torch_with_other_inner_names(ops, monkeypatch):      # noqa: F811
+    from test_row_ops_calls import without_private_names
+    other = without_private_names(monkeypatch)
+    x = torch.randn(3000, 64, device=DEV)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+        y = other.group_norm(x, 4, act="silu")
+    torch.cuda.synchronize()
+    assert torch.equal(y, ops.group_norm(x, 4, act="silu"))

@@ -97,3 +97,34 @@ def test_arguments_of_other_types_are_refused_by_name(here):
             call()
     import numpy as np
     assert row_ops._whole(np.int64(4), "groups") == 4 and row_ops._number(1, "eps") == 1.0 and row_ops._number(np.float32(0.5), "slope") == 0.5
+
+
+INSIDE_TORCH = ("_cuda_getCurrentRawStream", "_cuda_getDevice", "_is_tracing", "_len_torch_dispatch_stack", "_functorch")
+
+
+def without_private_names(monkeypatch):
+    """The module as it is on a torch whose inner names are others."""
+    import importlib.util
+    from lssvc_amd import row_ops
+
+    class Inner:
+        def __getattr__(self, name):
+            if name in INSIDE_TORCH:
+                raise AttributeError(name)
+            return getattr(inner, name)
+    inner = torch._C
+    monkeypatch.setattr(torch, "_C", Inner())
+    spec = importlib.util.spec_from_file_location("lssvc_amd.row_ops_elsewhere", row_ops.__file__)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    monkeypatch.setattr(torch, "_C", inner)
+    return module
+
+
+def test_the_module_does_not_need_names_inside_torch(monkeypatch):
+    module = without_private_names(monkeypatch)
+    assert module._current_device is torch.cuda.current_device and module._tracing is torch.jit.is_tracing
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index: type("S", (), {"cuda_stream": 7 + index}))
+    assert module._raw_stream(2) == 9
+    monkeypatch.setattr(module, "_current_device", lambda: 0)
+    assert module._elsewhere(torch.device("cuda:0")) is False and module._elsewhere(torch.device("cuda:1")) is True
