@@ -514,7 +514,7 @@ typedef struct lssvc_fp8 {
  * x holds images x (rows / images) rows. weight / bias: cols fp32 values or NULL (1 / 0). Exactly one of y (x's shape and type;
  * may be x itself) and y8 (1 x 128 blocks, e8m0 scales; the block's scale and values are those lssvc_quantize_fp8 makes of the
  * fp32 result) is given. rows = 0 is no work. workspace: lssvc_group_norm_workspace_bytes(...) bytes, 16-byte aligned, private to
- * the call until it has run; may be NULL where that is 0. */
+ * the call until it has run; may be NULL where that is 0 (as it also is for sizes that the call refuses). */
 int64_t lssvc_group_norm_workspace_bytes(int64_t rows, int32_t images, int32_t cols, int32_t groups, int32_t dtype, int32_t to_fp8);
 int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t groups, const float *weight, const float *bias, float eps,
                      int32_t act, float slope, const lssvc_rows *y, const lssvc_fp8 *y8, void *workspace, int64_t workspace_bytes,

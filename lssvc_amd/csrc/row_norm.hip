@@ -594,6 +594,11 @@ static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8)
     return q;
 }
 
+// Sizes within which the plan's and the workspace's arithmetic holds (an image's rows are counted in 32 bits; more images x columns than 2^40 values
+// fit no memory)
+static bool norm_range(int64_t rows, int64_t images, int64_t cols) {
+    return rows < (1LL << 40) && cols <= (1 << 30) && rows / images <= (1LL << 30) && images * cols <= (1LL << 40);
+}
 static int64_t norm_ws(const NormPlan &q, int images, int C, int G) {
     return q.resident ? 0 : 16 * (int64_t)images * q.S * G * q.P + 12 * (int64_t)images * C;
 }
@@ -685,7 +690,7 @@ int rows_check(const char *what, const lssvc_rows *x) {
 using namespace lssvc;
 
 extern "C" int64_t lssvc_group_norm_workspace_bytes(int64_t rows, int32_t images, int32_t cols, int32_t groups, int32_t dtype, int32_t to_fp8) {
-    if (rows <= 0 || images <= 0 || cols <= 0 || groups <= 0 || cols % groups || rows % images || !rows_type_ok(dtype)) return 0;
+    if (rows <= 0 || images <= 0 || cols <= 0 || groups <= 0 || cols % groups || rows % images || !rows_type_ok(dtype) || !norm_range(rows, images, cols)) return 0;
     return norm_ws(norm_plan(rows / images, images, cols, groups, rows_type_size(dtype), to_fp8 != 0), images, cols, groups);
 }
 
@@ -698,6 +703,7 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     LSSVC_CHECK(eps >= 0.f, "group_norm: eps %g", eps);
     LSSVC_CHECK(act_ok(act), "group_norm: unknown activation %d", act);
     LSSVC_CHECK((y != nullptr) != (y8 != nullptr), "group_norm: exactly one of the outputs is given");
+    LSSVC_CHECK(norm_range(x->rows, images, x->cols), "group_norm: %d images of %lld rows x %d channels are too large", images, (long long)(x->rows / images), x->cols);
     const int64_t R = x->rows / images;
     const NormPlan q = norm_plan(R, images, x->cols, groups, rows_type_size(x->dtype), y8 != nullptr);
     const int64_t need = x->rows ? norm_ws(q, images, x->cols, groups) : 0;
@@ -714,7 +720,7 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     } else LSSVC_CHECK(apart({ws}, {span_of(x)}), "group_norm: the workspace overlaps the input");
     if (x->rows == 0) return 0;
     LSSVC_CHECK(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), "group_norm: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need, (long long)workspace_bytes);
-    LSSVC_CHECK(R <= (1LL << 30) && q.P <= kMergeMax, "group_norm: an image of %lld rows x %d channels in %d groups is too large", (long long)R, x->cols, groups);
+    LSSVC_CHECK(q.P <= kMergeMax, "group_norm: an image of %lld rows x %d channels in %d groups is too large", (long long)R, x->cols, groups);
     LSSVC_CHECK((int64_t)images * std::max<int64_t>(groups, (int64_t)q.nslices * std::max(q.S, 1)) < (1LL << 31), "group_norm: too many images or groups for one launch");
     NormP p{};
     p.x = x->ptr;

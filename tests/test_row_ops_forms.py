@@ -9,3 +9,18 @@ def test_the_tile_query_refuses_what_the_product_refuses():
     t = lambda a, w, dtype=0, rows=r: _lib.lib.lssvc_matmul_fp8_tile(a, w, dtype, rows and C.byref(rows), C.byref(c))
     assert t(f(), f(32, br=128)) == 0 and (r.value, c.value) == (16, 16)
     assert t(f(), f(32)) != 0 and t(f(), f(32, 63, 128)) != 0 and t(f(), f(32, br=128, e8m0=0)) != 0 and t(f(), f(32, br=128), 3) != 0 and t(f(), f(32, br=128), 0, None) != 0
+
+
+def test_sizes_beyond_the_operators_range():
+    """The workspace's size of what no call takes is 0, not a number that has overflowed; the call says what is wrong."""
+    from lssvc_amd import _lib
+    size, big = _lib.lib.lssvc_group_norm_workspace_bytes, 2 ** 31 - 1
+    for args in ((8, 1, big, 1), (big, 1, big, big), (big, big, big, 1), (2 ** 40, 1, 64, 4), (2 ** 39, 1, 64, 4), (big, big, 2 ** 30, 2 ** 30), (2 ** 62, 2, 8, 8), (8, 1, 2 ** 30 + 1, 1)):
+        for dtype in (_lib.F32, _lib.BF16):
+            for fp8 in (0, 1):
+                assert size(*args, dtype, fp8) == 0, args
+    assert size(2 ** 30, 1, 64, 4, 0, 0) > 0 and size(60000, 1, 2 ** 20, 32, 0, 0) > 0
+    row = lambda rows, cols, at: C.byref(_lib.Rows(at, rows, cols, cols, 0))
+    for rows, images, cols in ((2 ** 39, 1, 64), (big, big, 2 ** 20)):
+        assert _lib.lib.lssvc_group_norm(row(rows, cols, 1 << 12), images, 1, None, None, 1e-5, 0, 0.0, row(rows, cols, 1 << 62), None, None, 0, None) != 0
+        assert b"too large" in _lib.lib.lssvc_last_error()
