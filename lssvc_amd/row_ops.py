@@ -91,7 +91,10 @@ def _vector(x, name, n, device):
         _refuse("row_ops: %s has to be %d adjacent fp32 values on %s", name, n, device)
     if x.requires_grad:
         _no_grad(x, name)
-    return x.data_ptr()
+    p = x.data_ptr()
+    if not p:                                                      # (a wrapper of another tensor; no address would mean no weight)
+        _refuse("row_ops: %s has no memory of its own: %s", name, type(x).__name__)
+    return p
 
 
 def _whole(v, name):

@@ -89,3 +89,24 @@ def test_on_a_torch_with_other_inner_names(ops, monkeypatch):      # noqa: F811
         y = other.group_norm(x, 4, act="silu")
     torch.cuda.synchronize()
     assert torch.equal(y, ops.group_norm(x, 4, act="silu"))
+
+
+def test_wrappers_without_memory_are_refused(ops):         # noqa: F811
+    """A tensor that only wraps others has the address 0, which to the library means no weight: it must not be left out in silence."""
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, t):
+            return torch.Tensor._make_wrapper_subclass(cls, t.shape, strides=t.stride(), dtype=t.dtype, device=t.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, f, types, args=(), kwargs=None):
+            raise RuntimeError("not looked into")
+    x, v = torch.randn(32, 64, device=DEV), torch.ones(64, device=DEV)
+    q, w = ops.quantize_fp8(x), ops.quantize_fp8(torch.randn(64, 64, device=DEV), 128)
+    wx, wv = Wrapper(x), Wrapper(v)
+    for call in (lambda: ops.group_norm(x, 4, wv), lambda: ops.group_norm(x, 4, None, wv), lambda: ops.group_norm_fp8(x, 4, wv), lambda: ops.matmul_fp8(q, w, wv),
+                 lambda: ops.group_norm(wx, 4), lambda: ops.quantize_fp8(wx), lambda: ops.matmul_fp8(q, w, residual=wx), lambda: ops.group_norm(x, 4, out=wx)):
+        with pytest.raises((ops.LssvcHipError, RuntimeError)):
+            call()
+    with pytest.raises(ops.LssvcHipError, match="no memory of its own"):
+        ops.group_norm(x, 4, wv)
