@@ -110,3 +110,22 @@ def test_wrappers_without_memory_are_refused(ops):         # noqa: F811
             call()
     with pytest.raises(ops.LssvcHipError, match="no memory of its own"):
         ops.group_norm(x, 4, wv)
+
+
+def test_scales_with_room_behind_a_row(ops):               # noqa: F811
+    """e8m0 scales of 2 and 5 blocks a row at a pitch of 4 and 8: read in place, whatever stands between the rows; without room for the last row's, copied."""
+    g = gen(9)
+    for m, n, k, pitch in ((40, 300, 200, 4), (1500, 1300, 600, 8), (1, 70, 130, 4)):
+        q, w = ops.quantize_fp8(torch.randn(m, k, generator=g).to(DEV)), ops.quantize_fp8(torch.randn(n, k, generator=g).to(DEV), 128)
+        want = ops.matmul_fp8(q, w)
+        store = torch.full((m, pitch), 255, dtype=torch.uint8, device=DEV)               # (NaN, were it used)
+        kb = q.scale.shape[1]
+        store[:, :kb] = q.scale.contiguous().view(torch.uint8)
+        scale = store.view(torch.float8_e8m0fnu)[:, :kb]
+        a = ops.Fp8Rows(q.values, scale)
+        assert a.scale.data_ptr() == store.data_ptr()
+        assert torch.equal(ops.matmul_fp8(a, w), want)
+        short = store.flatten()[:(m - 1) * pitch + kb].clone().as_strided((m, kb), (pitch, 1)).view(torch.float8_e8m0fnu)
+        a = ops.Fp8Rows(q.values, short)
+        assert a.scale.data_ptr() != short.data_ptr()
+        assert torch.equal(ops.matmul_fp8(a, w), want)

@@ -24,3 +24,16 @@ def test_sizes_beyond_the_operators_range():
     for rows, images, cols in ((2 ** 39, 1, 64), (big, big, 2 ** 20)):
         assert _lib.lib.lssvc_group_norm(row(rows, cols, 1 << 12), images, 1, None, None, 1e-5, 0, 0.0, row(rows, cols, 1 << 62), None, None, 0, None) != 0
         assert b"too large" in _lib.lib.lssvc_last_error()
+
+
+def test_scales_with_room_behind_a_row_are_read_in_place():
+    import torch
+    from lssvc_amd.row_ops import _whole_dwords
+    store = torch.zeros(64, dtype=torch.uint8)
+    at = lambda rows, kb, ld, off=0, step=1: store.as_strided((rows, kb), (ld, step), off).view(torch.float8_e8m0fnu)
+    for rows, kb, ld, off in ((4, 2, 4, 0), (1, 4, 4, 60), (1, 1, 99, 60), (16, 1, 4, 0), (15, 3, 4, 4), (3, 5, 8, 40), (2, 4, 60, 0), (1, 61, 64, 0)):
+        assert _whole_dwords(at(rows, kb, ld, off)), (rows, kb, ld, off)
+    for rows, kb, ld, off, step in ((4, 2, 2, 0, 1), (4, 2, 6, 0, 1), (1, 2, 4, 61, 1), (1, 2, 4, 62, 1), (4, 2, 4, 2, 1), (2, 2, 4, 58, 1), (4, 2, 0, 0, 1), (4, 3, 16, 0, 2), (4, 5, 4, 0, 1)):
+        assert not _whole_dwords(at(rows, kb, ld, off, step)), (rows, kb, ld, off, step)
+    short = torch.zeros(10, dtype=torch.uint8).as_strided((2, 2), (8, 1)).view(torch.float8_e8m0fnu)      # its last row ends with the memory
+    assert not _whole_dwords(short)
