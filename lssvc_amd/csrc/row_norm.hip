@@ -8,8 +8,8 @@
 //   split     rows are split over workgroups that write sums per chunk and group; the chunks are joined by a launch of their own, or, where
 //             they are few, by every workgroup of the normalising pass for itself; that pass reads the map again, in the opposite order,
 //             so that what the first pass read last comes from the caches.
-// Measured: 18x30x64 fp32 4.6 us (resident); 1152x1920x48 fp32 266 us = 113 (3.8 TB/s, what a read-only
-// pass reaches) + 5 + 148 (5.7 TB/s); 34560x256 bf16 to 8 bits 7.6 + 3.4 + 10.6 us, of which the activation and the encoding are half.
+// Measured: 18x30x64 fp32 4.2 us (resident); 1152x1920x48 fp32 266 us = 113 (3.8 TB/s, what a read-only
+// pass reaches) + 5 + 148 (5.7 TB/s); 34560x256 bf16 to 8 bits 7.5 + 3.5 + 10.7 us, of which the activation and the encoding are half.
 // Sums S1 = sum x and S2 = sum x^2 are in 64 bits from the first value on: squares of fp32 and bf16 values leave fp32's range (from 1.8e19 and
 // below 1e-19 on), and S2 - S1^2 / N keeps what fp32 data can hold: an offset a thousand times the spread costs 2^-33 of the variance. A value
 // costs a conversion, an addition and an FMA, which run at the rate of fp32 ones. The mean is held as two fp32 numbers, the second folded
@@ -152,7 +152,7 @@ template <int TPB, typename E, typename G, typename F> __device__ __forceinline_
         }
     }
 }
-// `hold(u)`: where S1 of a unit waits for S2 (8 bytes, the lane's own until then). `rows`: rows in flight that hold anything
+// `hold(u)` (TURNS only): where S1 of a unit waits for S2, 8 bytes, the lane's own until then. `rows`: rows in flight that hold anything
 template <int TPB, int V, Sums HOW, typename H, typename F>
 __device__ __forceinline__ void unit_sums(const double (&s1)[kChains<V, HOW>], const double (&s2)[kChains<V, HOW>], int rows, const Lane<V> &l, int nv, int sc, int uw, uint32_t m_uw, uint32_t m_w,
                                           int nu, void *entries, H hold, F done) {
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormP p) {
     }
     const int per = divided_any(rows, rp), rem = rows - per * rp;
     double2 *out = p.part + ((int64_t)img * p.G * p.P + (p.P == 1 ? divided_any(s0, p.cg) : sl)) * p.S + chunk;
-    unit_sums<TPB, V, HOW>(s1, s2, per > 0 ? rp : rem, l, nv, sc, uw, p.m_uw, m_w, nu, entries, [&](int u) { return &out[(int64_t)u * p.S].x; },
+    unit_sums<TPB, V, HOW>(s1, s2, per > 0 ? rp : rem, l, nv, sc, uw, p.m_uw, m_w, nu, entries, nullptr,
                            [&](int u, double a, double b) { out[(int64_t)u * p.S] = make_double2(a, b); });
 }
 

@@ -153,7 +153,7 @@ def _elsewhere(device, *tensors):
     if hip_ops.recording():
         _refuse("row_ops: not part of compiled frame plans")
     if device.index is None:
-        _refuse("row_ops: 8-bit rows on %s: there is no CPU path", device)
+        _refuse("row_ops: operands on %s: there is no CPU path", device)
     return device.index != _current_device()
 
 
@@ -321,8 +321,8 @@ def _group_norm(x, groups, weight, bias, eps, act, slope, images, out, fp8):
 
 
 def group_norm(x, groups, weight=None, bias=None, *, eps=1e-5, act=None, slope=0.01, images=None, out=None):
-    """act(group_norm(x)): statistics over the rows of each of `images` images and the C / groups channels of a group, sums in 64 bits (finite
-    values of any size and offset); weight / bias: C fp32 values. images: for 2-d rows and T (default 1); a 4-d tensor brings its own. out: rows of
+    """act(group_norm(x)): statistics over the rows of each of `images` images and the C / groups channels of a group, sums in 64 bits (values
+    up to 1e38, of any offset); weight / bias: C fp32 values. images: for 2-d rows and T (default 1); a 4-d tensor brings its own. out: rows of
     x's shape and type, x itself allowed. act: None, 'lrelu' (slope), 'relu', 'silu'."""
     return _group_norm(x, groups, weight, bias, eps, act, slope, images, out, False)
 
