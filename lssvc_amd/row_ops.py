@@ -236,7 +236,9 @@ class Fp8Rows:
     def dequantize(self, dtype=torch.float32):
         """The (rows, cols) values the blocks stand for, in plain torch operations (for inspection and tests)."""
         s = self.scale.contiguous()
-        s = s if s.dtype == torch.float32 else (s.view(torch.uint8).to(torch.int32) << 23).view(torch.float32)
+        if s.dtype != torch.float32:                               # 2^(b - 127) is the exponent field, but for the ends of the range
+            b = s.view(torch.uint8).to(torch.int32)
+            s = torch.where(b == 0, 0x400000, torch.where(b == 255, 0x7fc00000, b << 23)).to(torch.int32).view(torch.float32)
         s = s.repeat_interleave(self.block_rows, 0)[:self.rows].repeat_interleave(BLOCK, 1)[:, :self.cols]
         return (self.values.float() * s).to(dtype)
 

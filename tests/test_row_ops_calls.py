@@ -128,3 +128,15 @@ def test_the_module_does_not_need_names_inside_torch(monkeypatch):
     assert module._raw_stream(2) == 9
     monkeypatch.setattr(module, "_current_device", lambda: 0)
     assert module._elsewhere(torch.device("cuda:0")) is False and module._elsewhere(torch.device("cuda:1")) is True
+
+
+def test_dequantize_at_the_ends_of_the_scales():
+    """2^-127, which is no normal number, and the byte that stands for NaN."""
+    from lssvc_amd.row_ops import Fp8Rows
+    q = Fp8Rows.empty(4, 200, "cpu")
+    q.values[:] = torch.full((4, 200), 1.5).to(torch.float8_e4m3fn)
+    q.scale.view(torch.uint8)[:] = torch.tensor([[0, 1], [254, 255], [127, 126], [253, 2]], dtype=torch.uint8)
+    got = q.dequantize(torch.float64)
+    want = 1.5 * torch.exp2(torch.tensor([[-127.0, -126], [127, 0], [0, -1], [126, -125]], dtype=torch.float64))
+    want[1, 1] = float("nan")
+    assert torch.equal(got[:, 0].nan_to_num(7), want[:, 0]) and torch.equal(got[:, 199].nan_to_num(7), want[:, 1].nan_to_num(7))
