@@ -33,7 +33,7 @@ struct NormP {
     int64_t R;                   // rows of an image
     const float *w, *b;
     double2 *part;               // split form: [image][unit][chunk] (S1, S2): whole lines for those who add a unit up
-    float *mean, *scale, *shift; // split form: [image][channel] mean, weight / sqrt(var + eps), bias less the mean's second part
+    float *mean, *scale, *shift; // split form without join: [image][channel] mean, weight / sqrt(var + eps), bias less the mean's second part
     int64_t chunk;               // rows of a chunk
     int C, G, cg;
     int S;                       // chunks of an image
@@ -544,6 +544,7 @@ struct NormPlan {
     int slice, nslices, P, piece, S;
     int64_t chunk;
     Sums sums;
+    bool join;               // split: the normalising pass adds up the chunks itself
 };
 static int gcd_i(int a, int b) { return b ? gcd_i(b, a % b) : a; }
 constexpr int kMergeMax = 2048;          // chunks x pieces: what one merging workgroup adds up
@@ -591,6 +592,8 @@ static NormPlan norm_plan(int64_t R, int images, int C, int G, int es, bool to8)
     if (chunk < 8 * rp) chunk = 8 * rp;
     q.chunk = chunk;
     q.S = (int)((R + chunk - 1) / chunk);
+    // joining costs every workgroup of the last pass what it reads; a launch costs 3 us of the device's time and as much of the host's
+    q.join = (int64_t)q.S * q.P * G <= 1024;
     return q;
 }
 
@@ -600,7 +603,7 @@ static bool norm_range(int64_t rows, int64_t images, int64_t cols) {
     return rows < (1LL << 40) && cols <= (1 << 30) && rows / images <= (1LL << 30) && images * cols <= (1LL << 40);
 }
 static int64_t norm_ws(const NormPlan &q, int images, int C, int G) {
-    return q.resident ? 0 : 16 * (int64_t)images * q.S * G * q.P + 12 * (int64_t)images * C;
+    return q.resident ? 0 : 16 * (int64_t)images * q.S * G * q.P + (q.join ? 0 : 12 * (int64_t)images * C);
 }
 
 template <typename T, int V, int TPB, Sums HOW, bool TO8> static int launch_resident(const NormP &p, const NormPlan &q, int images, hipStream_t s) {
@@ -657,8 +660,7 @@ template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, 
     else if (q.sums == ONE) norm_stats_kernel<T, V, ONE><<<(unsigned)g1, 256, 0, s>>>(n);
     else if (q.sums == TWO) norm_stats_kernel<T, V, TWO><<<(unsigned)g1, 256, 0, s>>>(n);
     else norm_stats_kernel<T, V, EACH><<<(unsigned)g1, 256, 0, s>>>(n);
-    // joining costs every workgroup of the last pass what it reads; a launch costs 3 us of the device's time and as much of the host's
-    const bool join = (int64_t)q.S * q.P * p.G <= 1024;
+    const bool join = q.join;
     if (!join) norm_merge_kernel<<<(unsigned)g_merge, 256, 0, s>>>(p);
     n.nv = nv, n.m_nv = division_magic(nv);
     auto apply = [&](auto kernel) { kernel<<<(unsigned)g2, 256, 0, s>>>(n, sc, nsl, (int)S2, chunk2); };

@@ -37,3 +37,13 @@ def test_scales_with_room_behind_a_row_are_read_in_place():
         assert not _whole_dwords(at(rows, kb, ld, off, step)), (rows, kb, ld, off, step)
     short = torch.zeros(10, dtype=torch.uint8).as_strided((2, 2), (8, 1)).view(torch.float8_e8m0fnu)      # its last row ends with the memory
     assert not _whole_dwords(short)
+
+
+def test_workspace_holds_what_the_passes_hand_on():
+    """Sums of 16 bytes per chunk and group; per-channel values only where a pass of their own joins the chunks."""
+    from lssvc_amd import _lib
+    size = _lib.lib.lssvc_group_norm_workspace_bytes
+    assert size(3000, 3000, 8200, 1, _lib.F16, 0) == 16 * 3000 * 9                       # 9 pieces of a group, joined by the last pass
+    assert size(20000, 1, 200, 8, _lib.F32, 0) < 16 * 1024 * 8
+    many = size(1152 * 1920, 1, 48, 8, _lib.F32, 0)
+    assert many >= 12 * 48 and (many - 12 * 48) % (16 * 8) == 0 and many < 1 << 20
