@@ -612,7 +612,7 @@ template <typename T, int V, int TPB, Sums HOW, bool TO8> static int launch_resi
         if (int rc = grant.ensure((const void *)norm_resident_kernel<T, V, TPB, HOW, TO8>, kResidentBytes, 64 * 1024)) return rc;
     NormP n = p;
     const int rp = TPB / threads_of<V, TO8>(q.slice), its = (int)((p.R + rp - 1) / rp);
-    n.parts = p.in_place ? 1 : std::max(1, std::min(std::min(12, its), 256 / std::min(256, images * q.nslices)));
+    n.parts = p.in_place ? 1 : std::max(1, std::min(std::min(12, its), 256 / (int)std::min<int64_t>(256, (int64_t)images * q.nslices)));
     n.nv = threads_of<V, TO8>(q.slice), n.m_nv = division_magic(n.nv);
     n.m_uw = division_magic(p.cg), n.m_w = division_magic(entries_of(HOW, p.cg, V));
     const int64_t workgroups = (int64_t)images * q.nslices * n.parts;
@@ -670,6 +670,24 @@ template <typename T> static int launch_norm(const NormP &p, const NormPlan &q, 
     return launch_status("group_norm");
 }
 
+// All images: as many at a time as one launch's threads can be counted for (one-row images of 8 narrow slices: 2 million)
+template <typename T> static int launch_images(const NormP &p, const NormPlan &q, int images, bool to8, hipStream_t s) {
+    const int64_t sl2 = (p.C + 255) / 256;                     // (at least the last pass's slices)
+    const int64_t per = q.resident ? q.nslices : std::max<int64_t>(std::max<int64_t>((int64_t)q.nslices * q.S, sl2), q.join ? 0 : p.G);
+    const int most = (int)std::min<int64_t>(images, std::max<int64_t>(1, ((1LL << 32) - 1) / (q.resident ? q.tpb : 256) / per));
+    for (int64_t i = 0; i < images; i += most) {
+        NormP n = p;
+        const int64_t rows = i * p.R;
+        n.x = (const T *)p.x + rows * p.ldx;
+        if (to8) n.q = p.q + rows * p.ldq, n.qs = p.qs + rows * p.ldqs;
+        else n.y = (T *)p.y + rows * p.ldy;
+        n.part = p.part + i * q.S * p.G * q.P;
+        n.mean = p.mean + i * p.C, n.scale = p.scale + i * p.C, n.shift = p.shift + i * p.C;
+        if (int rc = launch_norm<T>(n, q, (int)std::min<int64_t>(most, images - i), to8, s)) return rc;
+    }
+    return 0;
+}
+
 int fp8_out_check(const char *what, const lssvc_fp8 *y, int64_t rows, int cols) {
     LSSVC_CHECK(y && (rows == 0 || (y->values && y->scale)), "%s: no 8-bit output", what);
     LSSVC_CHECK(y->rows == rows && y->cols == cols, "%s: 8-bit output is %lld x %d, expected %lld x %d", what, (long long)y->rows, y->cols, (long long)rows, cols);
@@ -723,7 +741,6 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     if (x->rows == 0) return 0;
     LSSVC_CHECK(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)), "group_norm: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need, (long long)workspace_bytes);
     LSSVC_CHECK(q.P <= kMergeMax, "group_norm: an image of %lld rows x %d channels in %d groups is too large", (long long)R, x->cols, groups);
-    LSSVC_CHECK((int64_t)images * std::max<int64_t>(groups, (int64_t)q.nslices * std::max(q.S, 1)) < (1LL << 31), "group_norm: too many images or groups for one launch");
     NormP p{};
     p.x = x->ptr;
     p.ldx = x->ld;
@@ -740,7 +757,7 @@ extern "C" int lssvc_group_norm(const lssvc_rows *x, int32_t images, int32_t gro
     p.scale = p.mean + (int64_t)images * x->cols;
     p.shift = p.scale + (int64_t)images * x->cols;
     hipStream_t s = (hipStream_t)stream;
-    if (x->dtype == LSSVC_F32) return launch_norm<float>(p, q, images, y8 != nullptr, s);
-    if (x->dtype == LSSVC_F16) return launch_norm<f16_t>(p, q, images, y8 != nullptr, s);
-    return launch_norm<bf16_t>(p, q, images, y8 != nullptr, s);
+    if (x->dtype == LSSVC_F32) return launch_images<float>(p, q, images, y8 != nullptr, s);
+    if (x->dtype == LSSVC_F16) return launch_images<f16_t>(p, q, images, y8 != nullptr, s);
+    return launch_images<bf16_t>(p, q, images, y8 != nullptr, s);
 }

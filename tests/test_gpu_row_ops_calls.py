@@ -129,3 +129,22 @@ def test_scales_with_room_behind_a_row(ops):               # noqa: F811
         a = ops.Fp8Rows(q.values, short)
         assert a.scale.data_ptr() != short.data_ptr()
         assert torch.equal(ops.matmul_fp8(a, w), want)
+
+
+@pytest.mark.parametrize("images,c,groups,dtype,fp8", [(2200000, 64, 8, torch.float32, False), (2200000, 1024, 64, torch.bfloat16, True), (1900000, 8200, 1, torch.float16, False)])
+def test_more_images_than_a_launch_holds(ops, images, c, groups, dtype, fp8):       # noqa: F811
+    """Every row an image of its own (a norm per pixel): more workgroups than a launch's threads can be counted for."""
+    few = 1000
+    rows = (torch.randn(few, c, generator=gen(c)) * 3 + 1).to(dtype).to(DEV)
+    want = ops.group_norm_fp8(rows, groups, act="relu", images=few) if fp8 else ops.group_norm(rows, groups, act="relu", images=few)
+    x = torch.empty(images, c, dtype=dtype, device=DEV)
+    x.view(images // few, few, c)[:] = rows
+    if fp8:
+        q = ops.group_norm_fp8(x, groups, act="relu", images=images)
+        same = lambda at: torch.equal(q.values[at].view(torch.uint8), want.values.view(torch.uint8)) and torch.equal(q.scale[at].view(torch.uint8), want.scale.view(torch.uint8))
+    else:
+        ops.group_norm(x, groups, act="relu", images=images, out=x)
+        same = lambda at: torch.equal(x[at], want)
+    for k in range(0, images // few, 50):
+        assert same(slice(k * few, (k + 1) * few)), k
+    assert same(slice(images - few, images))
